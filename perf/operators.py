@@ -119,7 +119,7 @@ def prepare(case, seed):
         # The expert weights as a program that serves them keeps them: 4-bit codes, two to a byte along K, and
         # scales in blocks of 128 rows by 4, in the order [.., row block, column block, row % 32, row // 32, column].
         codes, scale = _codes(randn(E, N, K) / math.sqrt(K))
-        c["data"] = (codes[..., 0::2] | (codes[..., 1::2] << 4)).contiguous()
+        c["data"] = (codes[..., 0::2] | (codes[..., 1::2] << 4)).to(torch.uint8).contiguous()
         rb, kb = -(-N // 128), -(-scale.shape[-1] // 4)
         full = torch.zeros(E, rb * 128, kb * 4, dtype=torch.uint8, device="cuda")
         full[:, :N, :scale.shape[-1]] = scale
