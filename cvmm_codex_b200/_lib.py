@@ -32,6 +32,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
 _S = ctypes.c_size_t
+_F = ctypes.c_float
 SIGNATURES = {
     "cvmm_abi_version": (_I, []),
     "cvmm_last_error": (ctypes.c_char_p, []),
@@ -64,6 +65,12 @@ SIGNATURES = {
                                _P, _P, _I, _L, _I, _P, _P, _S, _P]),
     "cvmm_gelu_backward": (_I, [_P, _P, _P, _I, _L, _P]),
     "cvmm_router_topk": (_I, [_P, _I, _L, _L, _L, _I, _P, _P, _P]),
+    "cvmm_router_select": (_I, [_P, _I, _L, _L, _L, _L, _I, _P, _I, _L, _L, _I, _I, _F, _P, _P, _P]),
+    "cvmm_router_select_backward": (_I, [_P, _I, _L, _P, _P, _L, _L, _L, _I, _I, _F, _P, _P]),
+    "cvmm_mx_quantize": (_I, [_P, _I, _L, _L, _L, _L, _L, _L, _P, _P, _P]),
+    "cvmm_mx_dequantize": (_I, [_P, _P, _L, _L, _L, _L, _L, _L, _P, _I, _P]),
+    "cvmm_mx_workspace_size": (_S, [_L, _L, _L, _L, _L]),
+    "cvmm_mx_forward": (_I, [_P, _I, _L, _L, _P, _I, _L, _L, _P, _I, _P, _P, _L, _L, _L, _P, _I, _P, _S, _P]),
 }
 
 _lib = None

@@ -19,7 +19,7 @@ fake implementation (cvmm.py:1442-1450).
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 
@@ -260,6 +260,65 @@ def _(logits, top_k, renormalize):
     return logits.new_empty(shape, dtype=torch.float32), logits.new_empty(shape, dtype=torch.int64)
 
 
+@torch.library.custom_op("cvmm_b200::router_select", mutates_args=())
+def router_select(logits: torch.Tensor, top_k: int, scoring: str, bias: Optional[torch.Tensor], n_groups: int,
+                  top_groups: int, group_score: str, renormalize: bool,
+                  scale: float) -> tuple[torch.Tensor, torch.Tensor]:
+    return ops.router_select(logits, top_k, scoring, bias, n_groups, top_groups, group_score, renormalize, scale)
+
+
+@router_select.register_fake
+def _(logits, top_k, scoring, bias, n_groups, top_groups, group_score, renormalize, scale):
+    shape = (*logits.shape[:-1], top_k)
+    return logits.new_empty(shape, dtype=torch.float32), logits.new_empty(shape, dtype=torch.int64)
+
+
+@torch.library.custom_op("cvmm_b200::router_select_backward", mutates_args=())
+def router_select_backward(logits: torch.Tensor, sel: torch.Tensor, grad_w: torch.Tensor, scoring: str,
+                           renormalize: bool, scale: float) -> torch.Tensor:
+    return ops.router_select_backward(logits, sel, grad_w, scoring, renormalize, scale)
+
+
+@router_select_backward.register_fake
+def _(logits, sel, grad_w, scoring, renormalize, scale):
+    return logits.new_empty(logits.shape)
+
+
+# ------------------------------------------------------------------ microscaled 4-bit tensors
+@torch.library.custom_op("cvmm_b200::mx_quantize", mutates_args=())
+def mx_quantize(x: torch.Tensor, dim: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return ops.mx_quantize(x, dim)
+
+
+@mx_quantize.register_fake
+def _(x, dim):
+    data, scale = ops.mx_shapes(x.shape, dim)
+    return x.new_empty(data, dtype=torch.uint8), x.new_empty(scale, dtype=torch.uint8)
+
+
+@torch.library.custom_op("cvmm_b200::mx_dequantize", mutates_args=())
+def mx_dequantize(data: torch.Tensor, scale: torch.Tensor, shape: Sequence[int], dim: int,
+                  dtype: torch.dtype) -> torch.Tensor:
+    return ops.mx_dequantize(data, scale, shape, dim, dtype)
+
+
+@mx_dequantize.register_fake
+def _(data, scale, shape, dim, dtype):
+    return data.new_empty(shape, dtype=dtype)
+
+
+@torch.library.custom_op("cvmm_b200::mx_forward", mutates_args=())
+def mx_forward(x: torch.Tensor, sel: torch.Tensor, keys_data: torch.Tensor, keys_scale: torch.Tensor, k_dim: int,
+               w: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
+    return ops.mx_forward(x, sel, keys_data, keys_scale, k_dim, w, out_dtype)
+
+
+@mx_forward.register_fake
+def _(x, sel, keys_data, keys_scale, k_dim, w, out_dtype):
+    lead = sel.shape if w is None else sel.shape[:-1]
+    return x.new_empty((*lead, keys_data.shape[1]), dtype=out_dtype)
+
+
 # ------------------------------------------------------------------ the reference's op schema
 @torch.library.custom_op("cvmm_b200::cvmm_triton", mutates_args=())
 def cvmm_triton(x: torch.Tensor, sel_index: torch.Tensor, sel: torch.Tensor, keys: torch.Tensor,
@@ -404,6 +463,29 @@ class _Calls:
         if self._tracing():
             return torch.ops.cvmm_b200.router_topk(logits, top_k, renormalize)
         return ops.router_topk(logits, top_k, renormalize)
+
+    def router_select(self, logits, top_k, scoring, bias, n_groups, top_groups, group_score, renormalize, scale):
+        fn = torch.ops.cvmm_b200.router_select if self._tracing() else ops.router_select
+        return fn(logits, top_k, scoring, bias, n_groups, top_groups, group_score, renormalize, scale)
+
+    def router_select_backward(self, logits, sel, grad_w, scoring, renormalize, scale):
+        fn = torch.ops.cvmm_b200.router_select_backward if self._tracing() else ops.router_select_backward
+        return fn(logits, sel, grad_w, scoring, renormalize, scale)
+
+    def mx_shapes(self, shape, dim):
+        return ops.mx_shapes(shape, dim)
+
+    def mx_quantize(self, x, dim):
+        fn = torch.ops.cvmm_b200.mx_quantize if self._tracing() else ops.mx_quantize
+        return fn(x, dim)
+
+    def mx_dequantize(self, data, scale, shape, dim, dtype):
+        fn = torch.ops.cvmm_b200.mx_dequantize if self._tracing() else ops.mx_dequantize
+        return fn(data, scale, shape, dim, dtype)
+
+    def mx_forward(self, x, sel, keys_data, keys_scale, k_dim, w, out_dtype):
+        fn = torch.ops.cvmm_b200.mx_forward if self._tracing() else ops.mx_forward
+        return fn(x, sel, keys_data, keys_scale, k_dim, w, out_dtype)
 
 
 calls = _Calls()

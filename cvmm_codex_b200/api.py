@@ -597,6 +597,64 @@ class _RouterTopK(torch.autograd.Function):
         return gl.to(logits.dtype), None, None
 
 
+def router_select(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias: Optional[torch.Tensor] = None,
+                  n_groups: int = 1, top_groups: Optional[int] = None, group_score: str = "max",
+                  renormalize: bool = True, scale: float = 1.0):
+    """(weights fp32, sel int64), both [..., top_k]: the experts of every token.
+
+    scoring: scores s = "softmax" or "sigmoid" of the logits [..., E] (fp32, bf16
+    or fp16). bias: [E], added to the scores for the choice alone (a balance
+    bias; it gets no gradient). n_groups > 1: the experts are groups of
+    E / n_groups consecutive ones, and only those of the top_groups groups
+    (default: all) with the largest value are eligible; group_score: "max" (a
+    group's largest biased score) or "top2" (the sum of its two largest). Of the
+    eligible experts the top_k with the largest biased score are chosen, in
+    descending order, ties to the lowest index; the order is that of 64-bit
+    scores. weights: the unbiased scores of the chosen, divided by their sum
+    when renormalize (held at 1e-20), times scale. Experts with logit -inf are
+    chosen after all others, with weight 0; NaN logits rank first and give NaN
+    weights. Differentiable once w.r.t. the logits. No reference counterpart
+    beyond softmax top-k (router_topk)."""
+    if logits.dim() < 1 or logits.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError(f"router_select: logits must be a float tensor [..., E], got {logits.dtype} {tuple(logits.shape)}")
+    if scoring not in ("softmax", "sigmoid"):
+        raise ValueError(f"router_select: scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
+    if group_score not in ("max", "top2"):
+        raise ValueError(f"router_select: group_score must be 'max' or 'top2', got {group_score!r}")
+    E = logits.shape[-1]
+    top_groups = n_groups if top_groups is None else top_groups
+    if not 1 <= E <= 1024:
+        raise ValueError(f"router_select: needs 1 to 1024 experts, got {E}")
+    if not 1 <= n_groups <= 32 or E % n_groups != 0 or not 1 <= top_groups <= n_groups:
+        raise ValueError(f"router_select: {n_groups} groups (at most 32, dividing {E} experts), {top_groups} of them chosen")
+    if not 1 <= top_k <= min(32, E // n_groups * top_groups):
+        raise ValueError(f"router_select: top_k {top_k} must be 1 to 32 and no more than the eligible experts")
+    if bias is not None:
+        if tuple(bias.shape) != (E,) or bias.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise ValueError(f"router_select: bias must be a float tensor [{E}], got {bias.dtype} {tuple(bias.shape)}")
+        if bias.device != logits.device:
+            raise ValueError(f"router_select: bias is on {bias.device}, logits on {logits.device}")
+        bias = bias.detach()
+    return _RouterSelect.apply(logits, int(top_k), scoring, bias, int(n_groups), int(top_groups), group_score,
+                               bool(renormalize), float(scale))
+
+
+class _RouterSelect(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_k, scoring, bias, n_groups, top_groups, group_score, renormalize, scale):
+        w, sel = ops.router_select(logits, top_k, scoring, bias, n_groups, top_groups, group_score, renormalize, scale)
+        ctx.save_for_backward(logits, sel)
+        ctx.how = (scoring, renormalize, scale)
+        ctx.mark_non_differentiable(sel)
+        return w, sel
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_w, grad_sel):
+        logits, sel = ctx.saved_tensors
+        return (ops.router_select_backward(logits, sel, grad_w, *ctx.how),) + (None,) * 8
+
+
 known_shapes = set()
 
 

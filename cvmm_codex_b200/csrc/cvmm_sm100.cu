@@ -6,3 +6,5 @@
 #include "sel_prep_noalloc.cu"
 #include "simt_gemm.cu"
 #include "umma_gemm.cu"
+#include "router.cu"
+#include "mx.cu"

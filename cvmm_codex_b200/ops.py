@@ -7,7 +7,7 @@ implementations so that torch.compile can trace through CVMM.
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 
@@ -21,6 +21,8 @@ KERNELS_PER_CALL = {
     "cvmm_backward_w": 4, "cvmm_weighted_combine": 1, "cvmm_sum_routes": 1,
     "cvmm_weighted_token_backward": 1, "cvmm_cast": 1, "cvmm_sort_rows_padded": 2, "cvmm_sort_rows_padded_ex": 2, "cvmm_pad_starts": 1,
     "cvmm_forward_gelu": 1, "cvmm_gelu_backward": 1, "cvmm_router_topk": 1, "cvmm_padded_route_rows": 1,
+    "cvmm_router_select": 1, "cvmm_router_select_backward": 1, "cvmm_mx_quantize": 1, "cvmm_mx_dequantize": 1,
+    "cvmm_mx_forward": 3,
 }
 
 
@@ -481,3 +483,126 @@ def router_topk(logits: torch.Tensor, top_k: int, renormalize: bool = True):
                      int(bool(renormalize)), ptr(sel), ptr(w), stream)
     check(rc, "cvmm_router_topk")
     return w, sel
+
+
+SCORING = {"softmax": 0, "sigmoid": 1}  # CVMM_SCORE_*
+GROUP_SCORE = {"max": 0, "top2": 1}  # CVMM_GROUP_*
+
+
+def router_select(logits: torch.Tensor, top_k: int, scoring: str, bias: Optional[torch.Tensor], n_groups: int,
+                  top_groups: int, group_score: str, renormalize: bool, scale: float):
+    """(weights fp32 [..., k], sel int64 [..., k]) of api.router_select, in one launch."""
+    _require_cuda(logits, bias)
+    lib = _lib.load()
+    lg = _rows(logits)
+    T, E = lg.shape
+    b = None if bias is None else bias.contiguous()
+    sel = torch.empty((*logits.shape[:-1], int(top_k)), dtype=torch.int64, device=lg.device)
+    w = torch.empty((*logits.shape[:-1], int(top_k)), dtype=torch.float32, device=lg.device)
+    with _Device(lg.device) as stream:
+        rc = _invoke("cvmm_router_select", lib.cvmm_router_select, ptr(lg), dtype_code(lg.dtype), lg.stride(0), T, E,
+                     int(top_k), SCORING[scoring], ptr(b), dtype_code(b.dtype) if b is not None else 0, int(n_groups),
+                     int(top_groups), GROUP_SCORE[group_score], int(bool(renormalize)), float(scale), ptr(sel), ptr(w),
+                     stream)
+    check(rc, "cvmm_router_select")
+    return w, sel
+
+
+def router_select_backward(logits: torch.Tensor, sel: torch.Tensor, grad_w: torch.Tensor, scoring: str,
+                           renormalize: bool, scale: float) -> torch.Tensor:
+    """Gradient of router_select's weights w.r.t. the logits (logits' shape and dtype)."""
+    _require_cuda(logits, sel, grad_w)
+    lib = _lib.load()
+    lg = _rows(logits)
+    T, E = lg.shape
+    s, g = sel.contiguous(), grad_w.float().contiguous()
+    out = torch.empty(logits.shape, dtype=lg.dtype, device=lg.device)
+    with _Device(lg.device) as stream:
+        rc = _invoke("cvmm_router_select_backward", lib.cvmm_router_select_backward, ptr(lg), dtype_code(lg.dtype),
+                     lg.stride(0), ptr(s), ptr(g), T, E, sel.shape[-1], SCORING[scoring], int(bool(renormalize)),
+                     float(scale), ptr(out), stream)
+    check(rc, "cvmm_router_select_backward")
+    return out
+
+
+# ------------------------------------------------------------------ microscaled 4-bit tensors
+def _mx_view(shape, dim: int):
+    """(batch, rows, K) of a logical shape quantised along dim."""
+    lead = 1
+    for n in shape[:dim]:
+        lead *= int(n)
+    return (1, lead, int(shape[-1])) if dim == -1 else (lead, int(shape[-1]), int(shape[-2]))
+
+
+def mx_shapes(shape, dim: int):
+    """Shapes of the data and scale tensors of a microscaled tensor (see cvmm_mx_quantize in the C header)."""
+    if dim not in (-1, -2) or len(shape) < -dim:
+        raise ValueError(f"microscaled tensors are quantised along dim -1 or -2 of their shape, got {dim} of {tuple(shape)}")
+    _, rows, K = _mx_view(shape, dim)
+    row_bytes = 16 * ((K + 31) // 32)
+    pieces = ((rows + 127) // 128, (K + 127) // 128, 32, 4, 4)
+    if dim == -1:
+        return (*shape[:-1], row_bytes), pieces
+    return (*shape[:-2], rows, row_bytes), (*shape[:-2], *pieces)
+
+
+def _mx_strides(t: torch.Tensor, dim: int):
+    """(t viewed as [batch, rows, K] or copied, (batch, row, k) strides in elements)."""
+    batch, rows, K = _mx_view(t.shape, dim)
+    if dim == -1:
+        v = t.reshape(rows, K)
+        return v, (0, v.stride(0), v.stride(1))
+    v = t.reshape(batch, K, rows)
+    return v, (v.stride(0), v.stride(2), v.stride(1))
+
+
+def mx_quantize(x: torch.Tensor, dim: int):
+    """(data uint8, scale uint8) of x quantised along dim (shapes: mx_shapes)."""
+    _require_cuda(x)
+    lib = _lib.load()
+    data_shape, scale_shape = mx_shapes(x.shape, dim)
+    batch, rows, K = _mx_view(x.shape, dim)
+    data = torch.empty(data_shape, dtype=torch.uint8, device=x.device)
+    scale = torch.empty(scale_shape, dtype=torch.uint8, device=x.device)
+    v, (sb, sr, sk) = _mx_strides(x, dim)
+    with _Device(x.device) as stream:
+        rc = _invoke("cvmm_mx_quantize", lib.cvmm_mx_quantize, ptr(v), dtype_code(v.dtype), batch, rows, K, sb, sr, sk,
+                     ptr(data), ptr(scale), stream)
+    check(rc, "cvmm_mx_quantize")
+    return data, scale
+
+
+def mx_dequantize(data: torch.Tensor, scale: torch.Tensor, shape: Sequence[int], dim: int,
+                  dtype: torch.dtype) -> torch.Tensor:
+    """The values of a microscaled tensor of logical `shape`, contiguous, in `dtype`."""
+    _require_cuda(data, scale)
+    lib = _lib.load()
+    batch, rows, K = _mx_view(shape, dim)
+    out = torch.empty(tuple(shape), dtype=dtype, device=data.device)
+    v, (sb, sr, sk) = _mx_strides(out, dim)
+    with _Device(data.device) as stream:
+        rc = _invoke("cvmm_mx_dequantize", lib.cvmm_mx_dequantize, ptr(data), ptr(scale), batch, rows, K, sb, sr, sk,
+                     ptr(v), dtype_code(dtype), stream)
+    check(rc, "cvmm_mx_dequantize")
+    return out
+
+
+def mx_forward(x: torch.Tensor, sel: torch.Tensor, keys_data: torch.Tensor, keys_scale: torch.Tensor, k_dim: int,
+               w: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
+    """The 4-bit expert product of mx.cvmm_mx: [*sel.shape, N], or [*sel.shape[:-1], N] with w."""
+    _require_cuda(x, sel, keys_data, keys_scale, w)
+    lib = _lib.load()
+    x2 = _rows(x)
+    E, N, K = keys_data.shape[0], keys_data.shape[1], int(k_dim)
+    s = sel.contiguous()
+    w2 = None if w is None else w.contiguous()
+    k, n_routes = s.shape[-1], s.numel()
+    out = torch.empty((*(s.shape if w is None else s.shape[:-1]), N), dtype=out_dtype, device=x.device)
+    ws = _ws(lib.cvmm_mx_workspace_size(x2.shape[0], n_routes, E, K, N), x.device)
+    with _Device(x.device) as stream:
+        rc = _invoke("cvmm_mx_forward", lib.cvmm_mx_forward, ptr(x2), dtype_code(x2.dtype), x2.shape[0], x2.stride(0),
+                     ptr(s), dtype_code(s.dtype), n_routes, k, ptr(w2), dtype_code(w2.dtype) if w2 is not None else 0,
+                     ptr(keys_data), ptr(keys_scale), E, K, N, ptr(out), dtype_code(out_dtype), ptr(ws), ws.numel(),
+                     stream)
+    check(rc, "cvmm_mx_forward")
+    return out

@@ -348,6 +348,71 @@ int cvmm_cast(const void* src, int src_dtype, void* dst, int dst_dtype, int64_t 
  * (the reference's in-kernel weight cast, cvmm.py:202-204). */
 int cvmm_cast_ahead(const void* src, int src_dtype, void* dst, int dst_dtype, int64_t n, cvmm_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Choosing experts beyond cvmm_router_topk: for every token with logits z,
+ *   s = softmax(z) or sigmoid(z);  c = s + bias  (bias NULL: the order of z);
+ *   with n_groups > 1 only the experts of the top_groups groups of
+ *   n_experts / n_groups consecutive experts with the largest value are
+ *   eligible (max: the largest c; top2: the sum of the two largest c, or s
+ *   without a bias);
+ *   sel = the top_k largest c, descending, ties to the lowest id;
+ *   weights_j = scale * s_j, divided by max(sum_j s_j, 1e-20) when renormalize.
+ * The order is that of c in 64 bits. An expert whose logit is -inf ranks below
+ * all others; a token with no other expert gets weights 0. NaN ranks first.
+ * logits: [n_tokens, n_experts] fp32/bf16/fp16 with leading dimension
+ * logits_ld; bias: [n_experts] fp32/bf16/fp16 or NULL; n_experts <= 1024,
+ * n_groups <= 32, top_k <= 32; sel int64, weights fp32, [n_tokens, top_k].
+ * No reference counterpart (its layer routes by softmax alone).
+ * ------------------------------------------------------------------------ */
+#define CVMM_SCORE_SOFTMAX 0
+#define CVMM_SCORE_SIGMOID 1
+#define CVMM_GROUP_MAX 0
+#define CVMM_GROUP_TOP2 1
+int cvmm_router_select(const void* logits, int logits_dtype, int64_t logits_ld, int64_t n_tokens, int64_t n_experts,
+                       int64_t top_k, int scoring, const void* bias, int bias_dtype, int64_t n_groups,
+                       int64_t top_groups, int group_score, int renormalize, float scale, int64_t* sel, float* weights,
+                       cvmm_stream_t stream);
+/* Gradient of weights w.r.t. the logits for the experts sel that
+ * cvmm_router_select chose (the choice itself and the bias have none).
+ * grad_weights: fp32 [n_tokens, top_k]; grad_logits: contiguous
+ * [n_tokens, n_experts] of logits_dtype, fully written. */
+int cvmm_router_select_backward(const void* logits, int logits_dtype, int64_t logits_ld, const int64_t* sel,
+                                const float* grad_weights, int64_t n_tokens, int64_t n_experts, int64_t top_k,
+                                int scoring, int renormalize, float scale, void* grad_logits, cvmm_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Microscaled 4-bit tensors [n_batch, rows, k_dim]: 32 values along k share the
+ * scale 2^(byte - 127), byte = 125 + floor(log2 max|v|) held to 0..254, 255
+ * (not a number) for a block with an infinity or NaN; a value is the nearest
+ * of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} times it (ties to even, held at 6).
+ *   data:  [n_batch, rows, 16 ceil(k_dim / 32)] bytes, two values to a byte,
+ *          the lower index in the lower half, zeros past k_dim;
+ *   scale: [n_batch, ceil(rows / 128), ceil(k_dim / 128), 32, 4, 4] bytes, row
+ *          r, block j at [r / 128][j / 4][r % 32][r % 128 / 32][j % 4]; padding 0.
+ * Both 16-byte aligned. x / out may have any strides (in elements); every byte
+ * of data and scale is written. No reference counterpart.
+ * ------------------------------------------------------------------------ */
+int cvmm_mx_quantize(const void* x, int x_dtype, int64_t n_batch, int64_t rows, int64_t k_dim, int64_t stride_b,
+                     int64_t stride_r, int64_t stride_k, uint8_t* data, uint8_t* scale, cvmm_stream_t stream);
+int cvmm_mx_dequantize(const uint8_t* data, const uint8_t* scale, int64_t n_batch, int64_t rows, int64_t k_dim,
+                       int64_t stride_b, int64_t stride_r, int64_t stride_k, void* out, int out_dtype,
+                       cvmm_stream_t stream);
+
+/* Expert product of 4-bit rows with 4-bit weights, for serving (no backward):
+ *   y[r] = Q(x[r / (n_routes / x_rows)]) . W[sel[r]]^T     fp32 accumulate
+ *   out[r] = y[r], or with w out[t] = sum_j w[t,j] y[t top_k + j]   (fp32 sum)
+ * Q quantises a row of x as cvmm_mx_quantize does. W is a microscaled tensor of
+ * n_experts x n_dim rows of k_dim (keys [E, k, n] quantised along k).
+ * x: [x_rows, k_dim] fp32/bf16/fp16 with leading dimension x_ld, x_rows a
+ * divisor of n_routes; sel: [n_routes] int64/int32 (an id outside
+ * [0, n_experts) contributes zeros and is reported in the status word);
+ * out: bf16/fp16, contiguous. */
+size_t cvmm_mx_workspace_size(int64_t x_rows, int64_t n_routes, int64_t n_experts, int64_t k_dim, int64_t n_dim);
+int cvmm_mx_forward(const void* x, int x_dtype, int64_t x_rows, int64_t x_ld, const void* sel, int sel_dtype,
+                    int64_t n_routes, int64_t top_k, const void* w, int w_dtype, const uint8_t* keys_data,
+                    const uint8_t* keys_scale, int64_t n_experts, int64_t k_dim, int64_t n_dim, void* out,
+                    int out_dtype, void* workspace, size_t workspace_bytes, cvmm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

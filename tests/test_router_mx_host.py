@@ -1,0 +1,141 @@
+"""Refusals and host-side shapes of router_select, mx_quantize and cvmm_mx (no GPU)."""
+import numpy as np
+import pytest
+import torch
+
+import cvmm_codex_b200 as b
+from cvmm_codex_b200 import _lib
+from cvmm_codex_b200.mx import mx_shapes
+from oracle import router_mx_oracle as O
+
+
+@pytest.mark.parametrize("bad", [
+    dict(top_k=0), dict(top_k=33), dict(top_k=9), dict(scoring="tanh"), dict(group_score="sum"), dict(n_groups=3),
+    dict(n_groups=0), dict(n_groups=4, top_groups=5), dict(n_groups=4, top_groups=0),
+    dict(n_groups=4, top_groups=1, top_k=3), dict(bias=torch.zeros(7)), dict(bias=torch.zeros(8, dtype=torch.int32)),
+    dict(bias=torch.zeros(8, dtype=torch.float64)), dict(bias=torch.zeros(1, 8)),
+])
+def test_router_select_refuses(bad):
+    args = dict(top_k=2)
+    args.update(bad)
+    with pytest.raises(ValueError, match="router_select"):
+        b.router_select(torch.zeros(4, 8), **args)
+
+
+@pytest.mark.parametrize("logits", [torch.zeros(4, 8, dtype=torch.float64), torch.zeros(4, 8, dtype=torch.int64),
+                                    torch.zeros(()), torch.zeros(4, 1025), torch.zeros(4, 0)])
+def test_router_select_refuses_logits(logits):
+    with pytest.raises(ValueError, match="router_select"):
+        b.router_select(logits, 1)
+
+
+def test_no_cpu_path():
+    with pytest.raises(RuntimeError, match="CUDA"):
+        b.router_select(torch.zeros(4, 8), 2)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        b.mx_quantize(torch.zeros(4, 8))
+
+
+def _keys(E=3, K=40, N=5):
+    data, scale = mx_shapes((E, K, N), -2)
+    return b.MXTensor(torch.zeros(data, dtype=torch.uint8), torch.zeros(scale, dtype=torch.uint8), (E, K, N), dim=-2)
+
+
+def test_mx_shapes():
+    assert mx_shapes((3, 40, 5), -2) == ((3, 5, 32), (3, 1, 1, 32, 4, 4))
+    assert mx_shapes((2, 300, 129), -1) == ((2, 300, 80), (5, 2, 32, 4, 4))
+    assert mx_shapes((7,), -1) == ((16,), (1, 1, 32, 4, 4))
+    for bad in (((7,), -2), ((2, 3), 0), ((2, 3), 1)):
+        with pytest.raises(ValueError):
+            mx_shapes(*bad)
+
+
+def test_mxtensor_refuses():
+    k = _keys()
+    for data, scale, shape, dim in (
+            (k.data.int(), k.scale, k.shape, -2), (k.data[:2], k.scale, k.shape, -2),
+            (k.data, k.scale[..., :3], k.shape, -2), (k.data, k.scale, (3, 5, 40), -1),
+            (k.data.mT.contiguous().mT, k.scale, k.shape, -2)):
+        with pytest.raises(ValueError, match="MXTensor|microscaled"):
+            b.MXTensor(data, scale, shape, dim)
+    with pytest.raises(ValueError, match="dtype"):
+        k.dequantize(torch.float64)
+
+
+def test_mx_quantize_refuses():
+    for x, dim in ((torch.zeros(4, 8, dtype=torch.float64), -1), (torch.zeros(4, 8), 0), (torch.zeros(4, 8), 1),
+                   (torch.zeros(8), -2)):
+        with pytest.raises(ValueError, match="mx_quantize"):
+            b.mx_quantize(x, dim)
+
+
+@pytest.mark.parametrize("x,sel,weights", [
+    (torch.zeros(4, 41), torch.zeros(4, 2, dtype=torch.int64), None),         # K
+    (torch.zeros(4, 40), torch.zeros(5, 2, dtype=torch.int64), None),         # tokens
+    (torch.zeros(4, 3, 40), torch.zeros(4, 2, dtype=torch.int64), None),      # rows that do not divide the routes
+    (torch.zeros(4, 40), torch.zeros(4, 2), None),                            # float ids
+    (torch.zeros(4, 40), torch.zeros(4, 0, dtype=torch.int64), None),
+    (torch.zeros(4, 40), torch.zeros((), dtype=torch.int64), None),
+    (torch.zeros(4, 40, dtype=torch.float64), torch.zeros(4, 2, dtype=torch.int64), None),
+    (torch.zeros(4, 40), torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, 3)),
+    (torch.zeros(4, 40), torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, 2, dtype=torch.int64)),
+])
+def test_cvmm_mx_refuses(x, sel, weights):
+    with pytest.raises(ValueError, match="cvmm_mx"):
+        b.cvmm_mx(x, sel, _keys(), weights)
+
+
+def test_cvmm_mx_refuses_keys_gradients_and_two_weights():
+    x, sel = torch.zeros(4, 40), torch.zeros(4, 2, dtype=torch.int64)
+    with pytest.raises(ValueError, match="keys"):
+        b.cvmm_mx(x, sel, torch.zeros(3, 40, 5))
+    data, scale = mx_shapes((3, 5, 40), -1)
+    rows = b.MXTensor(torch.zeros(data, dtype=torch.uint8), torch.zeros(scale, dtype=torch.uint8), (3, 5, 40), -1)
+    with pytest.raises(ValueError, match="keys"):
+        b.cvmm_mx(x, sel, rows)
+    with pytest.raises(RuntimeError, match="no backward"):
+        b.cvmm_mx(x.clone().requires_grad_(True), sel, _keys())
+    w = torch.ones(4, 2)
+    s = b.CVMMSel(sel.int(), sel.int(), sel.reshape(-1), None, w)
+    with pytest.raises(ValueError, match="twice"):
+        b.cvmm_mx(x, s, _keys(), w)
+
+
+@pytest.mark.parametrize("call,code", [
+    (lambda l: l.cvmm_router_select(16, 3, 8, 4, 8, 2, 0, None, 0, 1, 1, 0, 1, 1.0, 16, 16, None), -2),
+    (lambda l: l.cvmm_router_select(16, 0, 7, 4, 8, 2, 0, None, 0, 1, 1, 0, 1, 1.0, 16, 16, None), -1),
+    (lambda l: l.cvmm_router_select(16, 0, 8, 4, 8, 2, 2, None, 0, 1, 1, 0, 1, 1.0, 16, 16, None), -1),
+    (lambda l: l.cvmm_router_select(16, 0, 8, 4, 8, 2, 0, None, 0, 1, 1, 2, 1, 1.0, 16, 16, None), -1),
+    (lambda l: l.cvmm_router_select(16, 0, 8, 4, 8, 5, 0, None, 0, 4, 2, 0, 1, 1.0, 16, 16, None), -1),
+    (lambda l: l.cvmm_router_select(16, 0, 66, 4, 66, 2, 0, None, 0, 33, 2, 0, 1, 1.0, 16, 16, None), -1),
+    (lambda l: l.cvmm_router_select(None, 0, 8, 4, 8, 2, 0, None, 0, 1, 1, 0, 1, 1.0, 16, 16, None), -1),
+    (lambda l: l.cvmm_router_select_backward(16, 0, 8, 16, 16, 4, 8, 9, 0, 1, 1.0, 16, None), -1),
+    (lambda l: l.cvmm_router_select_backward(16, 0, 8, None, 16, 4, 8, 2, 0, 1, 1.0, 16, None), -1),
+    (lambda l: l.cvmm_mx_quantize(16, 3, 1, 4, 8, 0, 8, 1, 16, 16, None), -2),
+    (lambda l: l.cvmm_mx_quantize(16, 0, 1, -1, 8, 0, 8, 1, 16, 16, None), -1),
+    (lambda l: l.cvmm_mx_quantize(16, 0, 1, 4, 8, 0, 8, 1, 20, 16, None), -1),
+    (lambda l: l.cvmm_mx_dequantize(16, 16, 1, 4, 8, 0, 8, 1, None, 0, None), -1),
+    (lambda l: l.cvmm_mx_dequantize(16, 16, 1, 4, 8, 0, 8, 1, 16, 4, None), -2),
+    # out must be 16-bit; x rows must divide the routes; keys 16-byte aligned; a workspace is required
+    (lambda l: l.cvmm_mx_forward(16, 0, 4, 8, 16, 4, 8, 2, None, 0, 16, 16, 2, 8, 8, 16, 0, 16, 1 << 20, None), -2),
+    (lambda l: l.cvmm_mx_forward(16, 0, 3, 8, 16, 4, 8, 2, None, 0, 16, 16, 2, 8, 8, 16, 2, 16, 1 << 20, None), -1),
+    (lambda l: l.cvmm_mx_forward(16, 0, 4, 8, 16, 4, 8, 2, None, 0, 24, 16, 2, 8, 8, 16, 2, 16, 1 << 20, None), -1),
+    (lambda l: l.cvmm_mx_forward(16, 0, 4, 8, 16, 4, 8, 2, None, 0, 16, 16, 2, 8, 8, 16, 2, None, 0, None), -4),
+    (lambda l: l.cvmm_mx_forward(16, 0, 4, 8, 16, 0, 8, 2, None, 0, 16, 16, 2, 8, 8, 16, 2, 16, 1 << 20, None), -2),
+])
+def test_c_entries_refuse_before_any_launch(call, code):
+    lib = _lib.load()
+    assert call(lib) == code
+    assert len(lib.cvmm_last_error()) > 0
+
+
+def test_oracle_quantisation_is_nearest():
+    """The oracle itself: every value is within half a step of its grid, and the scale is the format's."""
+    x = np.random.default_rng(0).standard_normal((5, 70)) * np.exp(np.random.default_rng(1).standard_normal((5, 1)))
+    codes, scale = O.mx_quantize(x)
+    v = O.mx_values(codes, scale, 70)
+    s = np.exp2(scale.astype(float) - 127).repeat(32, -1)[:, :70]
+    a = np.abs(x) / s
+    step = np.where(a < 2, 0.5, np.where(a < 4, 1.0, 2.0))
+    assert (np.abs(v - x) / s <= np.where(a > 6, a - 6, step / 2)).all()
+    assert a.max() < 8
