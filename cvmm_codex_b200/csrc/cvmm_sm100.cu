@@ -8,3 +8,4 @@
 #include "umma_gemm.cu"
 #include "router.cu"
 #include "mx.cu"
+#include "mx_gemm.cu"

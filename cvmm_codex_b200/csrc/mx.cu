@@ -1,6 +1,5 @@
-// Microscaled 4-bit quantisation, its inverse, and the expert product of 4-bit
-// rows with 4-bit expert weights (cvmm_mx_quantize, cvmm_mx_dequantize,
-// cvmm_mx_forward). The layout is described in mx.cuh.
+// Microscaled 4-bit quantisation and its inverse (cvmm_mx_quantize,
+// cvmm_mx_dequantize). The layout is described in mx.cuh.
 #include "launch.h"
 #include "mx.cuh"
 
@@ -171,52 +170,6 @@ static int quantize(const void* x, int dtype, const View& v, uint8_t* data, uint
   return check_launch("cvmm_mx_quantize");
 }
 
-// ------------------------------------------------------------------ product
-// One thread an output value; the simplest form.
-__global__ void __launch_bounds__(256)
-product_kernel(const uint8_t* __restrict__ xd, const uint8_t* __restrict__ xs, int64_t per_row,
-               const void* __restrict__ sel, int sel_dtype, int64_t R, const uint8_t* __restrict__ kd,
-               const uint8_t* __restrict__ ks, int64_t E, int64_t K, int64_t N, float* __restrict__ y) {
-  pdl_enter();
-  const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
-  if (i >= R * N) return;
-  const int64_t r = i / N, n = i - r * N;
-  const int64_t e = sel_dtype == CVMM_I64 ? static_cast<const int64_t*>(sel)[r] : static_cast<const int32_t*>(sel)[r];
-  float acc = 0.f;
-  if (e < 0 || e >= E) {
-    if (n == 0) report(CVMM_DEV_BAD_INDEX, 31, (long long)e);
-  } else {
-    const int64_t rb = row_bytes(K), kp = pieces(K), row = r / per_row;
-    const uint8_t* ws = ks + e * scale_bytes(N, K);
-    for (int64_t j = 0; j * 32 < K; ++j) {
-      float part = 0.f;
-      for (int h = 0; h < 4; ++h) {
-        float a[8], b[8];
-        unpack8(*reinterpret_cast<const uint32_t*>(xd + row * rb + j * 16 + h * 4), a);
-        unpack8(*reinterpret_cast<const uint32_t*>(kd + (e * N + n) * rb + j * 16 + h * 4), b);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) part = fmaf(a[q], b[q], part);
-      }
-      acc += part * scale_value(xs[scale_cell(row, j >> 2, kp) + (j & 3)]) *
-             scale_value(ws[scale_cell(n, j >> 2, kp) + (j & 3)]);
-    }
-  }
-  y[i] = acc;
-}
-
-__global__ void __launch_bounds__(256) finish_kernel(const float* __restrict__ y, const void* __restrict__ w,
-                                                     int w_dtype, int64_t T, int64_t k, int64_t N,
-                                                     void* __restrict__ out, int dtype) {
-  pdl_enter();
-  const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
-  if (i >= T * N) return;
-  const int64_t t = i / N, n = i - t * N;
-  float acc = 0.f;
-  for (int64_t j = 0; j < k; ++j)
-    acc = fmaf(w ? load_as_float(w, w_dtype, t * k + j) : 1.f, y[(t * k + j) * N + n], acc);
-  store_from_float(out, dtype, i, acc);
-}
-
 }  // namespace mx
 }  // namespace cvmm
 
@@ -255,50 +208,6 @@ int cvmm_mx_dequantize(const uint8_t* data, const uint8_t* scale, int64_t n_batc
            scale, v, out, out_dtype);
   }
   return check_launch("cvmm_mx_dequantize");
-}
-
-size_t cvmm_mx_workspace_size(int64_t x_rows, int64_t n_routes, int64_t n_experts, int64_t k_dim, int64_t n_dim) {
-  using namespace cvmm;
-  (void)n_experts;
-  if (x_rows < 0 || n_routes < 0 || k_dim < 0 || n_dim < 0) return 0;
-  return align_up((size_t)(x_rows * mx::row_bytes(k_dim)), 256) + align_up((size_t)mx::scale_bytes(x_rows, k_dim), 256) +
-         align_up((size_t)(n_routes * n_dim) * 4, 256) + 256;
-}
-
-int cvmm_mx_forward(const void* x, int x_dtype, int64_t x_rows, int64_t x_ld, const void* sel, int sel_dtype,
-                    int64_t n_routes, int64_t top_k, const void* w, int w_dtype, const uint8_t* keys_data,
-                    const uint8_t* keys_scale, int64_t n_experts, int64_t k_dim, int64_t n_dim, void* out,
-                    int out_dtype, void* workspace, size_t workspace_bytes, cvmm_stream_t stream) {
-  using namespace cvmm;
-  if (!is_float_dtype(x_dtype) || (w && !is_float_dtype(w_dtype)) || (out_dtype != CVMM_BF16 && out_dtype != CVMM_F16))
-    return fail(CVMM_ERR_UNSUPPORTED_DTYPE, "cvmm_mx_forward: x and w must be float tensors, out bf16 or fp16");
-  if (sel_dtype != CVMM_I64 && sel_dtype != CVMM_I32)
-    return fail(CVMM_ERR_UNSUPPORTED_DTYPE, "cvmm_mx_forward: sel must be int64 or int32");
-  if (x_rows < 0 || n_routes < 0 || top_k < 1 || n_experts < 1 || n_experts > 65535 || k_dim < 1 || n_dim < 1 ||
-      x_ld < k_dim || n_routes % top_k != 0 || (n_routes > 0 && (x_rows < 1 || n_routes % x_rows != 0)))
-    return fail(CVMM_ERR_INVALID_ARG, "cvmm_mx_forward: bad sizes");
-  if (n_routes == 0) return CVMM_OK;
-  if (n_routes > (int64_t)INT32_MAX || k_dim > (int64_t)INT32_MAX || n_dim > (int64_t)INT32_MAX)
-    return fail(CVMM_ERR_INVALID_ARG, "cvmm_mx_forward: more than 2^31 routes, k or n");
-  if (!x || !sel || !keys_data || !keys_scale || !out)
-    return fail(CVMM_ERR_INVALID_ARG, "cvmm_mx_forward: null pointer");
-  if (!al16(keys_data) || !al16(keys_scale))
-    return fail(CVMM_ERR_INVALID_ARG, "cvmm_mx_forward: keys must be 16-byte aligned");
-  if (!workspace || workspace_bytes < cvmm_mx_workspace_size(x_rows, n_routes, n_experts, k_dim, n_dim))
-    return fail(CVMM_ERR_WORKSPACE, "cvmm_mx_forward: workspace too small");
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  uint8_t* ws = reinterpret_cast<uint8_t*>(align_up((size_t)workspace, 256));
-  uint8_t* xd = ws;
-  uint8_t* xs = xd + align_up((size_t)(x_rows * mx::row_bytes(k_dim)), 256);
-  float* y = reinterpret_cast<float*>(xs + align_up((size_t)mx::scale_bytes(x_rows, k_dim), 256));
-  const mx::View v = {1, x_rows, k_dim, 0, x_ld, 1};
-  if (int rc = mx::quantize(x, x_dtype, v, xd, xs, s)) return rc;
-  launch(mx::product_kernel, (unsigned)((n_routes * n_dim + 255) / 256), 256, 0, s, xd, xs, n_routes / x_rows, sel,
-         sel_dtype, n_routes, keys_data, keys_scale, n_experts, k_dim, n_dim, y);
-  const int64_t T = w ? n_routes / top_k : n_routes;
-  launch(mx::finish_kernel, (unsigned)((T * n_dim + 255) / 256), 256, 0, s, y, w, w_dtype, T, w ? top_k : 1, n_dim,
-         out, out_dtype);
-  return check_launch("cvmm_mx_forward");
 }
 
 }  // extern "C"

@@ -270,6 +270,27 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64
       : "memory");
 }
 
+// D[tmem] (+)= A[smem] * B[smem] with a scale for every 32 values along K of
+// each row (kind::mxf4: 4-bit e2m1 operands, two to a byte, K = 64; 8-bit
+// exponent scales in tensor memory at sa / sb; fp32 accumulate).
+__device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t sa, uint32_t sb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+          d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+      : "memory");
+}
+
+// 32 rows of 16 bytes (512 consecutive bytes of shared memory) into 4 columns
+// of lanes 0..31, repeated in every 32-lane quarter of tensor memory. Ordered
+// before the MMAs this thread issues after it.
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t s_desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
+}
+
 // Arrive on `bar` once every tcgen05 op previously issued by this thread completes.
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile(
@@ -308,6 +329,21 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo
   d |= (uint64_t)1u << 46;
   d |= (uint64_t)2u << 61;
   return d;
+}
+
+// Shared-memory matrix descriptor without swizzle: 8-row groups of 16-byte
+// rows, 128 bytes apart (layout = 0).
+__device__ __forceinline__ uint64_t smem_desc_rows16(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)8u << 32 | (uint64_t)1u << 46;
+}
+
+// Instruction descriptor for kind::mxf4, both operands K-major e2m1 (format 1),
+// scales of 8-bit exponents: [4,6) B scale byte, [7,10) A format, [10,13) B
+// format, [17,23) N >> 3, [23] exponent scales, [24,29) M >> 4, [29,31) A scale
+// byte. `byte` is where in its 4-byte column a K = 64 step's two scales start (0 or 2).
+__host__ __device__ constexpr uint32_t instr_desc_mxf4(int m, int n, int byte) {
+  return ((uint32_t)byte << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) |
+         ((uint32_t)(m >> 4) << 24) | ((uint32_t)byte << 29);
 }
 
 // Instruction descriptor for kind::f16 with fp32 accumulation:

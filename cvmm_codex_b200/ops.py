@@ -598,7 +598,7 @@ def mx_forward(x: torch.Tensor, sel: torch.Tensor, keys_data: torch.Tensor, keys
     w2 = None if w is None else w.contiguous()
     k, n_routes = s.shape[-1], s.numel()
     out = torch.empty((*(s.shape if w is None else s.shape[:-1]), N), dtype=out_dtype, device=x.device)
-    ws = _ws(lib.cvmm_mx_workspace_size(x2.shape[0], n_routes, E, K, N), x.device)
+    ws = _ws(lib.cvmm_mx_workspace_size(x2.shape[0], n_routes, E, K, N, int(w is not None)), x.device)
     with _Device(x.device) as stream:
         rc = _invoke("cvmm_mx_forward", lib.cvmm_mx_forward, ptr(x2), dtype_code(x2.dtype), x2.shape[0], x2.stride(0),
                      ptr(s), dtype_code(s.dtype), n_routes, k, ptr(w2), dtype_code(w2.dtype) if w2 is not None else 0,

@@ -404,10 +404,11 @@ int cvmm_mx_dequantize(const uint8_t* data, const uint8_t* scale, int64_t n_batc
  * Q quantises a row of x as cvmm_mx_quantize does. W is a microscaled tensor of
  * n_experts x n_dim rows of k_dim (keys [E, k, n] quantised along k).
  * x: [x_rows, k_dim] fp32/bf16/fp16 with leading dimension x_ld, x_rows a
- * divisor of n_routes; sel: [n_routes] int64/int32 (an id outside
+ * divisor of n_routes; n_experts <= 4096; sel: [n_routes] int64/int32 (an id outside
  * [0, n_experts) contributes zeros and is reported in the status word);
  * out: bf16/fp16, contiguous. */
-size_t cvmm_mx_workspace_size(int64_t x_rows, int64_t n_routes, int64_t n_experts, int64_t k_dim, int64_t n_dim);
+size_t cvmm_mx_workspace_size(int64_t x_rows, int64_t n_routes, int64_t n_experts, int64_t k_dim, int64_t n_dim,
+                              int weighted);
 int cvmm_mx_forward(const void* x, int x_dtype, int64_t x_rows, int64_t x_ld, const void* sel, int sel_dtype,
                     int64_t n_routes, int64_t top_k, const void* w, int w_dtype, const uint8_t* keys_data,
                     const uint8_t* keys_scale, int64_t n_experts, int64_t k_dim, int64_t n_dim, void* out,

@@ -156,7 +156,8 @@ def test_product_matches_64_bit(dtype, weighted, rows, T, K, N, E, k):
 
 
 @pytest.mark.parametrize("T,K,N,E,k,weighted", [(2000, 512, 320, 8, 3, False), (1500, 256, 640, 64, 8, True),
-                                                 (4, 4096, 136, 3, 2, True)])
+                                                 (4, 4096, 136, 3, 2, True),
+                                                 (9000, 160, 104, 8, 3, False), (9000, 544, 128, 5, 3, True)])
 def test_product_larger(T, K, N, E, k, weighted):
     x, keys, sel, w = make(T, K, N, E, k, torch.bfloat16, seed=5)
     check_product(x, keys, sel, w if weighted else None)
