@@ -82,7 +82,148 @@ __device__ __forceinline__ void unpack8(uint32_t p, float (&v)[8]) {
   }
 }
 
+// n / d by a multiplication for n < 2^31 (m = floor(2^(31 + l) / d) + 1 with
+// l = ceil(log2 d) is at most d / 2^(31 + l) too large, and n times that stays
+// below one); larger n divide.
+struct Divisor {
+  uint32_t d, m, l;
+  __host__ explicit Divisor(int64_t by) : d((uint32_t)by), m(0), l(0) {
+    while (((uint64_t)1 << l) < d) ++l;
+    if (d > 1) m = (uint32_t)((((uint64_t)1 << (31 + l)) / d) + 1);
+  }
+  __device__ __forceinline__ int64_t of(int64_t n) const {
+    if (d == 1) return n;
+    if (n >> 31) return n / d;
+    return __umulhi((uint32_t)n, m) >> (l - 1);
+  }
+};
+
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// 32 consecutive values of one type as the words they are loaded in.
+template <int DT>
+constexpr int kWords = DT == F32 ? 32 : 16;
+
+// 32-byte accesses (address a multiple of 32).
+__device__ __forceinline__ void ld_v8(uint32_t* w, const void* p) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void st_v8(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+// Loads values `at` .. at + 31 of x (those past n are 0). vec: bytes that the
+// address is a multiple of (32, 16, else value by value).
+template <int DT>
+__device__ __forceinline__ void load_block(uint32_t (&w)[kWords<DT>], const void* x, int64_t at, int n, int vec) {
+  constexpr int W = kWords<DT>;
+  const char* from = static_cast<const char*>(x) + at * (DT == F32 ? 4 : 2);
+  if (n >= 32 && vec == 32) {
+#pragma unroll
+    for (int i = 0; i < W; i += 8) ld_v8(w + i, from + 4 * i);
+  } else if (n >= 32 && vec == 16) {
+#pragma unroll
+    for (int i = 0; i < W; i += 4) {
+      const uint4 q = *reinterpret_cast<const uint4*>(from + 4 * i);
+      w[i] = q.x; w[i + 1] = q.y; w[i + 2] = q.z; w[i + 3] = q.w;
+    }
+  } else if (DT == F32) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = i < n ? reinterpret_cast<const uint32_t*>(from)[i] : 0u;
+  } else {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(from);
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      w[i] = (2 * i < n ? h[2 * i] : 0u) | (uint32_t)(2 * i + 1 < n ? h[2 * i + 1] : 0u) << 16;
+  }
+}
+
+// Magnitude bits (as a 32-bit float's) of the largest of 32 values: the bits of
+// a type order its magnitudes, infinities and NaN above the rest.
+template <int DT>
+__device__ __forceinline__ uint32_t block_magnitude(const uint32_t (&w)[kWords<DT>]) {
+  uint32_t m = 0;
+  if (DT == F32) {
+#pragma unroll
+    for (int i = 0; i < kWords<DT>; ++i) m = max(m, w[i] & 0x7fffffffu);
+    return m;
+  }
+#pragma unroll
+  for (int i = 0; i < kWords<DT>; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+  m = max(m & 0xffffu, m >> 16);
+  return DT == BF16 ? m << 16 : __float_as_uint(__half2float(__ushort_as_half((uint16_t)m)));
+}
+
+template <int DT>
+__device__ __forceinline__ uint4 pack_block(const uint32_t (&w)[kWords<DT>], float inv) {
+  uint32_t out[4];
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (DT == F32) f[j] = __uint_as_float(w[8 * h + j]);
+      else f[j] = bits_to_float((uint16_t)(j & 1 ? w[4 * h + j / 2] >> 16 : w[4 * h + j / 2] & 0xffffu), DT);
+    }
+    out[h] = pack8(f, inv);
+  }
+  return make_uint4(out[0], out[1], out[2], out[3]);
+}
+
+// Quantises blocks of rows whose K is contiguous, a lane a block, so that a
+// scale needs no other lane and a row's data go out 16 bytes a lane; four lanes
+// put a 4-byte cell of scales together. at(i) gives block i; blocks of a cell
+// are consecutive and start at a multiple of 4. `first` is blocks before this
+// thread's, `stride` blocks of a round. Every lane has its loads of kBlocks
+// rounds in flight before it converts any.
+struct Block {
+  int64_t src;     // element offset of the row's first value
+  uint8_t* data;   // the row's data bytes
+  uint32_t* cell;  // where the four scales go
+  int64_t j;       // which block of the row
+  bool row;        // false: a padding row, scales 0 and no data
+};
+
+template <int DT, class At>
+__device__ __forceinline__ void quantize_blocks(const void* __restrict__ x, int64_t K, int vec, int64_t items,
+                                                int64_t first, int64_t stride, At at) {
+  constexpr int kBlocks = DT == F32 ? 1 : 2;
+  const int lane4 = threadIdx.x & 3;
+  // Every lane of a warp runs the same number of rounds (shuffles below).
+  const int64_t rounds = (items + stride * kBlocks - 1) / (stride * kBlocks);
+  for (int64_t i = 0; i < rounds; ++i) {
+    uint32_t w[kBlocks][kWords<DT>];
+    Block q[kBlocks];
+#pragma unroll
+    for (int u = 0; u < kBlocks; ++u) {
+      const int64_t it = first + (i * kBlocks + u) * stride;
+      q[u] = at(it < items ? it : 0);
+      const int64_t left = it < items && q[u].row ? K - q[u].j * 32 : 0;
+      load_block<DT>(w[u], x, q[u].src + q[u].j * 32, (int)imin64(left, 32), vec);
+    }
+#pragma unroll
+    for (int u = 0; u < kBlocks; ++u) {
+      const bool live = first + (i * kBlocks + u) * stride < items;
+      const bool in = live && q[u].row && q[u].j * 32 < K;  // this block exists
+      const uint32_t byte = in ? scale_byte(block_magnitude<DT>(w[u])) : 0u;
+      if (in) *reinterpret_cast<uint4*>(q[u].data + q[u].j * 16) = pack_block<DT>(w[u], inverse_scale(byte));
+      uint32_t cell = byte << (8 * lane4);
+      cell |= __shfl_xor_sync(0xffffffffu, cell, 1);
+      cell |= __shfl_xor_sync(0xffffffffu, cell, 2);
+      if (live && lane4 == 0) *q[u].cell = cell;
+    }
+  }
+}
+
+// The largest of 32, 16 and 0 that an address, and steps of a and b bytes from it, are multiples of.
+inline int vector_bytes(const void* p, int64_t a, int64_t b) {
+  const uint64_t bits = (uint64_t)(uintptr_t)p | (uint64_t)a | (uint64_t)b;
+  return bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : 0;
+}
 
 }  // namespace mx
 }  // namespace cvmm

@@ -7,8 +7,8 @@
 //   prepare  quantises the rows of x once, in their own order (4 bits a value,
 //            so that all route copies of a row are reads of the same bytes), and
 //            lists the routes of every expert and the 128-route tiles they make;
-//   fill     (many routes only) writes the lists that prepare counted;
-//   gemm     gathers a tile's rows with TMA and multiplies them with the
+//   fill     (many routes only) writes the lists that prepare laid out;
+//   gemm     gathers a tile's rows and multiplies them with the
 //            expert's weight tiles on the tensor cores, scales and all;
 //   combine  (weights only) sums the route outputs.
 // The order of the routes within an expert's list is left to atomics: a row's
@@ -23,7 +23,7 @@ namespace mx {
 constexpr int kTile = 128;           // routes of a tile (MMA M)
 constexpr int64_t kMaxExperts = 4096;
 constexpr int kPlanThreads = 256;
-constexpr int64_t kPlanChunk = 4096;  // routes one block counts or lists
+constexpr int64_t kPlanChunk = 2048;  // routes one block ranks
 constexpr int kBadIdTag = 31;         // status-word site: an expert id outside [0, n_experts)
 enum : int { kTagEmpty = 40, kTagFull = 41, kTagAccFull = 42, kTagAccEmpty = 43, kTagDrain = 44 };
 
@@ -32,7 +32,7 @@ struct Product {
   const void* x;
   int x_dtype;
   int64_t x_rows, x_ld;
-  bool x_vec;
+  int x_vec;
   int per_row;  // routes that share a row
   uint8_t* xd;  // [x_rows][row_bytes]
   uint8_t* xs;  // [x_rows][cells] of 4 scale bytes, cells a multiple of 4
@@ -42,10 +42,11 @@ struct Product {
   int sel_dtype;
   int64_t R;
   int E;
-  int* header;   // [0] tiles, [1] blocks that have counted
-  int* cursor;   // [E] counts, then the next free place of every expert's list
+  int* header;   // [0] tiles, [1] blocks that have ranked their routes
+  int* cursor;   // [E] counts, then the start of every expert's list
   int4* tiles;   // (expert, first place in list, routes, -)
   int32_t* list; // routes by expert
+  int2* rank;    // (expert, place in its list) of every route, when several blocks rank
   // weights and output
   const uint8_t* kd;
   const uint8_t* ks;
@@ -105,10 +106,32 @@ __device__ void plan_tiles(const Product& p, int* counts, int* tstart, int* scra
   __syncthreads();
 }
 
-// Block 0 .. plan_blocks - 1 count (and, alone, list) routes; the others
-// quantise x: 16 lanes take 128 values of a row as quantize_k_kernel does, but
-// scale cells stay in row order, which is how a gathered tile reads them.
-__global__ void __launch_bounds__(kPlanThreads) prepare_kernel(const Product p, int plan_blocks) {
+// The up to kPer routes of a thread in a block of kPlanChunk: their experts, -1
+// for none or an id out of range (reported and zeroed, once a call).
+constexpr int kPer = (int)(kPlanChunk / kPlanThreads);
+__device__ __forceinline__ void my_routes(const Product& p, int64_t r0, int (&e)[kPer]) {
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int64_t r = r0 + threadIdx.x + j * kPlanThreads;
+    int64_t v = -1;
+    if (r < p.R) {
+      v = expert_of(p, r);
+      if (v < 0 || v >= p.E) {
+        bad_route(p, r, v);
+        v = -1;
+      }
+    }
+    e[j] = (int)v;
+  }
+}
+
+// Blocks 0 .. plan_blocks - 1 rank their routes within their experts; the last
+// of them to finish lays out the lists and tiles (and a lone one writes its
+// list, too). The other blocks quantise x; scale cells stay in row order,
+// which is how a gathered tile reads them.
+template <int DT>
+__global__ void __launch_bounds__(kPlanThreads)
+prepare_kernel(const __grid_constant__ Product p, int plan_blocks, Divisor by_blocks) {
   pdl_enter();
   extern __shared__ int sh[];  // counts[E], tstart[E + 1], 34 ints of scratch
   const int t = threadIdx.x;
@@ -116,114 +139,79 @@ __global__ void __launch_bounds__(kPlanThreads) prepare_kernel(const Product p, 
     int* counts = sh;
     int* tstart = sh + p.E;
     int* scratch = tstart + p.E + 1;
-    for (int e = t; e < p.E; e += kPlanThreads) counts[e] = 0;
+    const int64_t r0 = blockIdx.x * kPlanChunk;
+    int e[kPer], rank[kPer];
+    my_routes(p, r0, e);
+    for (int i = t; i < p.E; i += kPlanThreads) counts[i] = 0;
     __syncthreads();
-    const int64_t r0 = blockIdx.x * kPlanChunk, r1 = imin64(r0 + kPlanChunk, p.R);
-    for (int64_t r = r0 + t; r < r1; r += kPlanThreads) {
-      const int64_t e = expert_of(p, r);
-      if (e >= 0 && e < p.E) atomicAdd(&counts[e], 1);
-    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) rank[j] = e[j] >= 0 ? atomicAdd(&counts[e[j]], 1) : 0;
     __syncthreads();
     if (plan_blocks == 1) {
       plan_tiles(p, counts, tstart, scratch);
-      for (int64_t r = r0 + t; r < r1; r += kPlanThreads) {
-        const int64_t e = expert_of(p, r);
-        if (e >= 0 && e < p.E) p.list[atomicAdd(&counts[e], 1)] = (int32_t)r;
-        else bad_route(p, r, e);
-      }
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (e[j] >= 0) p.list[counts[e[j]] + rank[j]] = (int32_t)(r0 + t + j * kPlanThreads);
       return;
     }
-    for (int e = t; e < p.E; e += kPlanThreads)
-      if (counts[e]) atomicAdd(&p.cursor[e], counts[e]);
+    // This block's places within every expert's list.
+    for (int i = t; i < p.E; i += kPlanThreads)
+      if (counts[i]) counts[i] = atomicAdd(&p.cursor[i], counts[i]);
     __threadfence();
     __syncthreads();
     if (t == 0) scratch[32] = atomicAdd(&p.header[1], 1);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int64_t r = r0 + t + j * kPlanThreads;
+      if (r < p.R) p.rank[r] = e[j] >= 0 ? make_int2(e[j], counts[e[j]] + rank[j]) : make_int2(-1, 0);
+    }
     __syncthreads();
     if (scratch[32] != plan_blocks - 1) return;
     __threadfence();
-    for (int e = t; e < p.E; e += kPlanThreads) counts[e] = __ldcg(&p.cursor[e]);
+    for (int i = t; i < p.E; i += kPlanThreads) counts[i] = __ldcg(&p.cursor[i]);
     __syncthreads();
     plan_tiles(p, counts, tstart, scratch);
-    for (int e = t; e < p.E; e += kPlanThreads) p.cursor[e] = counts[e];
+    for (int i = t; i < p.E; i += kPlanThreads) p.cursor[i] = counts[i];
     return;
   }
-  const int64_t rb = row_bytes(p.K), items = p.x_rows * p.cells;
-  const int sub = t & 15;
-  const int64_t stride = (int64_t)(gridDim.x - plan_blocks) * (kPlanThreads / 16);
-  const int64_t rounds = (items + stride - 1) / stride;
-  for (int64_t i = 0; i < rounds; ++i) {
-    const int64_t it = (int64_t)(blockIdx.x - plan_blocks) * (kPlanThreads / 16) + (t >> 4) + i * stride;
-    const bool live = it < items;
-    const int64_t r = live ? it / p.cells : 0, c = live ? it - r * p.cells : 0;
-    const int64_t k0 = c * 128 + sub * 8;
-    float f[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = 0.f;
-    if (live && k0 < p.K) {
-      const int64_t at = r * p.x_ld + k0;
-      if (p.x_vec && k0 + 8 <= p.K) {
-        load8(static_cast<const char*>(p.x) + at * dtype_bytes(p.x_dtype), p.x_dtype, f);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (k0 + j < p.K) f[j] = load_as_float(p.x, p.x_dtype, at + j);
-      }
-    }
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, magnitude(f[j]));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const bool in = live && c * 128 + (sub & 12) * 8 < p.K;
-    const uint32_t byte = in ? scale_byte(m) : 0u;
-    if (in) *reinterpret_cast<uint32_t*>(p.xd + r * rb + k0 / 2) = pack8(f, inverse_scale(byte));
-    uint32_t cell = byte << (8 * ((sub >> 2) & 3));
-    cell |= __shfl_xor_sync(0xffffffffu, cell, 4);
-    cell |= __shfl_xor_sync(0xffffffffu, cell, 8);
-    if (live && sub == 0) *reinterpret_cast<uint32_t*>(p.xs + it * 4) = cell;
-  }
+  const int64_t rb = row_bytes(p.K), blocks = by_blocks.d;  // 4 a cell
+  auto at = [&](int64_t it) -> Block {
+    const int64_t r = by_blocks.of(it);
+    return {r * p.x_ld, p.xd + r * rb, reinterpret_cast<uint32_t*>(p.xs + (it & ~(int64_t)3)), it - r * blocks, true};
+  };
+  quantize_blocks<DT>(p.x, p.K, p.x_vec, p.x_rows * blocks,
+                      (int64_t)(blockIdx.x - plan_blocks) * kPlanThreads + t,
+                      (int64_t)(gridDim.x - plan_blocks) * kPlanThreads, at);
 }
 
-// Lists the routes counted by prepare: a block reserves its places of every
-// expert at once and hands them out in shared memory.
-__global__ void __launch_bounds__(kPlanThreads) fill_kernel(const Product p) {
+// Writes the lists that several blocks of prepare ranked.
+__global__ void __launch_bounds__(256) fill_kernel(const __grid_constant__ Product p) {
   pdl_enter();
-  extern __shared__ int sh[];  // counts[E]
-  const int t = threadIdx.x;
-  for (int e = t; e < p.E; e += kPlanThreads) sh[e] = 0;
-  __syncthreads();
-  const int64_t r0 = blockIdx.x * kPlanChunk, r1 = imin64(r0 + kPlanChunk, p.R);
-  for (int64_t r = r0 + t; r < r1; r += kPlanThreads) {
-    const int64_t e = expert_of(p, r);
-    if (e >= 0 && e < p.E) atomicAdd(&sh[e], 1);
-  }
-  __syncthreads();
-  for (int e = t; e < p.E; e += kPlanThreads)
-    if (sh[e]) sh[e] = atomicAdd(&p.cursor[e], sh[e]);
-  __syncthreads();
-  for (int64_t r = r0 + t; r < r1; r += kPlanThreads) {
-    const int64_t e = expert_of(p, r);
-    if (e >= 0 && e < p.E) p.list[atomicAdd(&sh[e], 1)] = (int32_t)r;
-    else bad_route(p, r, e);
-  }
+  const int64_t r = blockIdx.x * 256ll + threadIdx.x;
+  if (r >= p.R) return;
+  const int2 er = p.rank[r];
+  if (er.x >= 0) p.list[p.cursor[er.x] + er.y] = (int32_t)r;
 }
 
 // ------------------------------------------------------------------ gemm
 // Persistent, one CTA an SM, tiles of 128 routes x BN columns round-robin.
-//   warp 0      gathers the tile's rows: 4 rows x 128 bytes (256 values) an
-//               instruction, only the lanes that have rows;
-//   warp 1      gathers their scale cells, 16 bytes a row ahead in registers,
-//               and lays them out as tensor memory wants them: lane l takes rows
-//               l, l + 32, l + 64, l + 96, whose cells are 16 consecutive bytes;
-//   warp 2      lane 0 loads the weight tile (TMA) and its scales (bulk copies
+//   warps 0-3   gather the tile's rows, 16 bytes a copy into the 128-byte
+//               swizzle, and their scale cells, 4 bytes a copy into the order
+//               tensor memory wants (row r's at 16 (r % 32) + 4 (r / 32)); only
+//               rows that exist. The copies arrive on the stage's barrier by
+//               themselves. (Gathers by TMA, 4 rows an instruction, took 567 us
+//               where plain rows took 403, 32768 tokens 4096 -> 512.)
+//   warp 4      lane 0 loads the weight tile (TMA) and its scales (bulk copies
 //               of whole 512-byte pieces);
-//   warp 3      allocates tensor memory; lane 0 copies each stage's scales there
+//   warp 5      allocates tensor memory; lane 0 copies each stage's scales there
 //               (their own columns for every stage, so a copy never meets an MMA
 //               that still reads) and issues the MMAs, K = 64 each;
-//   warps 4-11  two groups read half the accumulator's columns each, round and
-//               store them through shared memory in 64-byte row pieces.
-constexpr int kThreads = 384;
-constexpr int kEpilogueWarps = 8;
+//   warps 6-13  two groups read half the accumulator's columns each, round them
+//               into registers, hand the accumulator back and only then store,
+//               through shared memory in 64-byte row pieces.
+constexpr int kProducers = 128;
+constexpr int kLoadWarp = 4, kMmaWarp = 5, kEpilogueWarp = 6, kEpilogueWarps = 8;
+constexpr int kThreads = 32 * (kEpilogueWarp + kEpilogueWarps);
 constexpr uint32_t kStagePitch = 80;  // 64-byte row piece + 16: 16-byte accesses meet no bank twice
 
 template <int BN, int S, int NACC>
@@ -244,24 +232,22 @@ struct Layout {
   static_assert(alloc <= 232448, "shared memory");
 };
 
-// One warp's 32 rows x 32 columns, rounded to 16 bits: lane l holds row l,
-// `off` its first element (-1: none). ncols is the same for the whole warp.
-__device__ __forceinline__ void store_rows(uint16_t* y, int dtype, int64_t off, const float (&v)[32], int ncols,
-                                           uint32_t stage, bool vec) {
+// One warp's 32 rows x 32 columns of 16-bit values, two to a word: lane l holds
+// row l, `off` its first element (-1: none). ncols is the same for the whole warp.
+__device__ __forceinline__ void store_rows(uint16_t* y, int64_t off, const uint32_t* v, int ncols, uint32_t stage,
+                                           bool vec) {
   const int lane = threadIdx.x & 31;
   if (!vec || ncols < 32) {
     if (off >= 0) {
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        if (j < ncols) y[off + j] = float_to_bits(v[j], dtype);
+        if (j < ncols) y[off + j] = (uint16_t)(j & 1 ? v[j >> 1] >> 16 : v[j >> 1] & 0xffffu);
     }
     return;
   }
 #pragma unroll
   for (int q = 0; q < 4; ++q)
-    ptx::st_shared_v4(stage + lane * kStagePitch + 16 * q, pack2(v[8 * q], v[8 * q + 1], dtype),
-                      pack2(v[8 * q + 2], v[8 * q + 3], dtype), pack2(v[8 * q + 4], v[8 * q + 5], dtype),
-                      pack2(v[8 * q + 6], v[8 * q + 7], dtype));
+    ptx::st_shared_v4(stage + lane * kStagePitch + 16 * q, v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
   __syncwarp();
   const int q = lane & 3;
 #pragma unroll
@@ -277,8 +263,7 @@ __device__ __forceinline__ void store_rows(uint16_t* y, int dtype, int64_t off, 
 
 template <int BN, int S, int NACC>
 __global__ void __launch_bounds__(kThreads, 1)
-gemm_kernel(const Product p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-            int n_n) {
+gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ CUtensorMap map_b, int n_n) {
   using L = Layout<BN, S, NACC>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = umma::align_smem(smem_raw);
@@ -292,7 +277,7 @@ gemm_kernel(const Product p, const __grid_constant__ CUtensorMap map_a, const __
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      ptx::mbar_init(&full[s], 3);  // rows, their scales, the weight tile
+      ptx::mbar_init(&full[s], kProducers + 1);  // the rows' copies, the weight tile
       ptx::mbar_init(&empty[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -303,7 +288,7 @@ gemm_kernel(const Product p, const __grid_constant__ CUtensorMap map_a, const __
     *abort = 0;
     ptx::fence_mbar_init();
   }
-  if (warp == 3) {
+  if (warp == kMmaWarp) {
     ptx::tmem_alloc(const_cast<uint32_t*>(tmem_slot), L::cols);
     ptx::tmem_relinquish();
   }
@@ -317,107 +302,54 @@ gemm_kernel(const Product p, const __grid_constant__ CUtensorMap map_a, const __
   auto tile = [&](int tt) -> int4 { return tt < total ? p.tiles[tt / n_n] : make_int4(0, 0, 0, 0); };
   const uint32_t base = ptx::smem_u32(smem);
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ rows
-    auto rows_of = [&](const int4& u, int (&r)[4]) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int i = 4 * lane + q;
-        r[q] = i < u.z ? (int)((uint32_t)p.list[u.y + i] / (uint32_t)p.per_row) : -1;
-      }
+  if (warp < 4) {
+    // ------------------------------------------------------------ rows and their scales
+    // Thread t copies 16-byte piece t % 8 of rows t / 8 + 16 i, and the scales
+    // of row t. The next tile's rows are looked up during the current tile.
+    const int t = threadIdx.x, piece = (t & 7) * 16;
+    auto row_of = [&](const int4& u, int i) -> int {
+      return i < u.z ? (int)((uint32_t)p.list[u.y + i] / (uint32_t)p.per_row) : -1;
     };
-    int4 u = tile(blockIdx.x);
-    int rows[4], next[4];
-    rows_of(u, rows);
+    int rows[8], next[8], srow, snext;
+    auto look = [&](const int4& u, int (&r)[8], int& sr) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = row_of(u, (t >> 3) + 16 * i);
+      sr = row_of(u, t);
+    };
+    look(tile(blockIdx.x), rows, srow);
     uint32_t it = 0;
     bool ok = true;
     for (int tt = blockIdx.x; tt < total && ok; tt += gridDim.x) {
-      const int4 un = tile(tt + gridDim.x);
-      rows_of(un, next);
-      const int lanes = (u.z + 3) / 4;
+      look(tile(tt + gridDim.x), next, snext);
+      const uint8_t* src[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) src[i] = p.xd + (int64_t)max(rows[i], 0) * rb + piece;
+      const uint8_t* scales = p.xs + (int64_t)max(srow, 0) * p.cells * 4;
       for (int kb = 0; kb < nkb; ++kb, ++it) {
         const int s = it % S;
         if (it >= S && !ptx::mbar_wait_or_abort(&empty[s], ((it / S) - 1) & 1, kTagEmpty, abort)) {
           ok = false;
           break;
         }
-        if (lane == 0) ptx::mbar_arrive_expect_tx(&full[s], lanes * 512);
-        __syncwarp();
-        if (lane < lanes)
-          ptx::tma_gather4(base + s * L::stage + lane * 512, &map_a, &full[s], kb * 128, rows[0], rows[1], rows[2],
-                           rows[3]);
-      }
-      u = un;
+        const uint32_t a_u = base + s * L::stage;
+        const bool in = kb * 128 + piece < rb;  // past the row's end: zeros
 #pragma unroll
-      for (int q = 0; q < 4; ++q) rows[q] = next[q];
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ scales of the rows
-    // Loads run three 16-byte chunks (of 512 values, two stages) ahead of the
-    // stores, across tiles, so that their latency hides behind the stages.
-    const int chunks = (nkb + 1) / 2;
-    const uint4* src[4];
-    int4 lu;                 // tile of the next load
-    int lt = blockIdx.x, lc = 0;
-    auto open = [&]() {
-      lu = tile(lt);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int i = lane + 32 * q;
-        src[q] = i < lu.z ? reinterpret_cast<const uint4*>(
-                                p.xs + (int64_t)((uint32_t)p.list[lu.y + i] / (uint32_t)p.per_row) * p.cells * 4)
-                          : nullptr;
-      }
-    };
-    auto load = [&](uint4 (&v)[4]) {
-      if (lt >= total) return;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] = src[q] ? src[q][lc] : make_uint4(0, 0, 0, 0);
-      if (++lc == chunks) {
-        lc = 0;
-        lt += gridDim.x;
-        if (lt < total) open();
-      }
-    };
-    uint4 v0[4] = {}, v1[4] = {}, v2[4] = {};
-    if (lt < total) open();
-    load(v0);
-    load(v1);
-    load(v2);
-    uint32_t it = 0;
-    bool ok = true;
-    for (int tt = blockIdx.x; tt < total && ok; tt += gridDim.x) {
-      for (int c = 0; c < chunks && ok; ++c) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (2 * c + h >= nkb) break;
-          const int s = it % S;
-          if (it >= S && !ptx::mbar_wait_or_abort(&empty[s], ((it / S) - 1) & 1, kTagEmpty, abort)) {
-            ok = false;
-            break;
-          }
-          const uint32_t dst = base + L::sa + s * 2 * kPiece + lane * 16;
-          if (h == 0) {
-            ptx::st_shared_v4(dst, v0[0].x, v0[1].x, v0[2].x, v0[3].x);
-            ptx::st_shared_v4(dst + kPiece, v0[0].y, v0[1].y, v0[2].y, v0[3].y);
-          } else {
-            ptx::st_shared_v4(dst, v0[0].z, v0[1].z, v0[2].z, v0[3].z);
-            ptx::st_shared_v4(dst + kPiece, v0[0].w, v0[1].w, v0[2].w, v0[3].w);
-          }
-          ptx::fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(&full[s]);
-          ++it;
+        for (int i = 0; i < 8; ++i)
+          if (rows[i] >= 0)
+            ptx::cp_async_16(a_u + umma::swz((t >> 3) + 16 * i, t & 7, 0), in ? src[i] + kb * 128 : p.xd, in ? 16 : 0);
+        if (srow >= 0) {
+          const uint32_t dst = base + L::sa + s * 2 * kPiece + (t & 31) * 16 + (t >> 5) * 4;
+          ptx::cp_async_4(dst, scales + kb * 8);
+          ptx::cp_async_4(dst + kPiece, scales + kb * 8 + 4);
         }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          v0[q] = v1[q];
-          v1[q] = v2[q];
-        }
-        load(v2);
+        ptx::cp_async_arrive_noinc(&full[s]);
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) rows[i] = next[i];
+      srow = snext;
     }
-  } else if (warp == 2) {
+    ptx::cp_async_wait_all();
+  } else if (warp == kLoadWarp) {
     // ------------------------------------------------------------ weight tiles
     if (lane == 0) {
       const int np_all = (int)pieces(p.N);
@@ -446,7 +378,7 @@ gemm_kernel(const Product p, const __grid_constant__ CUtensorMap map_a, const __
       }
     }
     __syncwarp();
-  } else if (warp == 3) {
+  } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMAs
     if (lane == 0) {
       const int np_all = (int)pieces(p.N);
@@ -466,6 +398,7 @@ gemm_kernel(const Product p, const __grid_constant__ CUtensorMap map_a, const __
             break;
           }
           ptx::tc_fence_after();
+          ptx::fence_proxy_async_smem();  // the rows came through the generic proxy
           const uint32_t sa = tmem + NACC * BN + s * L::sf_cols, sb = sa + 8;
           const int pc = min(2, kp - 2 * kb);
           for (int c = 0; c < pc; ++c) {
@@ -496,8 +429,8 @@ gemm_kernel(const Product p, const __grid_constant__ CUtensorMap map_a, const __
     __syncwarp();
   } else {
     // ------------------------------------------------------------ epilogue
-    const int quad = warp & 3, group = (warp - 4) >> 2;
-    const uint32_t stage = base + L::staging + (warp - 4) * 32 * kStagePitch;
+    const int quad = warp & 3, group = (warp - kEpilogueWarp) >> 2;
+    const uint32_t stage = base + L::staging + (warp - kEpilogueWarp) * 32 * kStagePitch;
     auto route_of = [&](const int4& u) -> int {
       const int i = quad * 32 + lane;
       return i < u.z ? p.list[u.y + i] : -1;
@@ -507,19 +440,27 @@ gemm_kernel(const Product p, const __grid_constant__ CUtensorMap map_a, const __
     for (int tt = blockIdx.x; tt < total; tt += gridDim.x, ++local) {
       const int route_next = route_of(tile(tt + gridDim.x));
       const int a = local % NACC;
-      const int64_t n0 = (int64_t)(tt % n_n) * BN;
+      const int64_t n0 = (int64_t)(tt % n_n) * BN + group * (BN / 2);
       if (!ptx::mbar_wait_or_abort(&accf[a], (local / NACC) & 1, kTagAccFull, abort)) break;
       ptx::tc_fence_after();
-      const int64_t off = route < 0 ? -1 : (int64_t)route * p.N + n0;
-      for (int c = group * (BN / 2); c < (group + 1) * (BN / 2); c += 32) {
-        if (n0 + c >= p.N) break;
-        float v[32];
-        umma::load_acc32(tmem + ((uint32_t)(quad * 32) << 16) + a * BN + c, v);
-        store_rows(p.y, p.out_dtype, off < 0 ? -1 : off + c, v, (int)imin64(32, p.N - n0 - c), stage, p.y_vec);
+      uint32_t v[BN / 4];
+#pragma unroll
+      for (int c = 0; c < BN / 64; ++c) {
+        if (n0 + 32 * c >= p.N) break;
+        float f[32];
+        umma::load_acc32(tmem + ((uint32_t)(quad * 32) << 16) + a * BN + group * (BN / 2) + 32 * c, f);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[16 * c + j] = pack2(f[2 * j], f[2 * j + 1], p.out_dtype);
       }
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&acce[a]);
+      const int64_t off = route < 0 ? -1 : (int64_t)route * p.N + n0;
+#pragma unroll
+      for (int c = 0; c < BN / 64; ++c) {
+        if (n0 + 32 * c >= p.N) break;
+        store_rows(p.y, off < 0 ? -1 : off + 32 * c, v + 16 * c, (int)imin64(32, p.N - n0 - 32 * c), stage, p.y_vec);
+      }
       route = route_next;
     }
   }
@@ -530,7 +471,7 @@ gemm_kernel(const Product p, const __grid_constant__ CUtensorMap map_a, const __
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 1000000) __nanosleep(1000);
   }
-  if (warp == 3) {
+  if (warp == kMmaWarp) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, L::cols);
   }
@@ -578,18 +519,7 @@ combine_kernel(const uint16_t* __restrict__ y, const void* __restrict__ w, int w
 }
 
 // ------------------------------------------------------------------ host side
-// Byte maps of 128-byte pieces (256 values) in the 128-byte swizzle.
-static bool rows_map(CUtensorMap* map, const void* base, int64_t rb, int64_t rows) {
-  auto fn = umma::encode_fn();
-  if (!fn) return false;
-  cuuint64_t dims[2] = {(cuuint64_t)rb, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)rb};
-  cuuint32_t box[2] = {128, 1}, estr[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
+// Byte map of the weights: boxes of 128 bytes (256 values) x bn rows in the 128-byte swizzle.
 static bool weights_map(CUtensorMap* map, const void* base, int64_t rb, int64_t N, int64_t E, int bn) {
   auto fn = umma::encode_fn();
   if (!fn) return false;
@@ -604,19 +534,19 @@ static bool weights_map(CUtensorMap* map, const void* base, int64_t rb, int64_t 
 template <int BN, int S, int NACC>
 static int launch_gemm(const Product& p, int64_t max_tiles, cudaStream_t stream) {
   using L = Layout<BN, S, NACC>;
-  CUtensorMap a, b;
-  if (!rows_map(&a, p.xd, row_bytes(p.K), p.x_rows) || !weights_map(&b, p.kd, row_bytes(p.K), p.N, p.E, BN))
+  CUtensorMap b;
+  if (!weights_map(&b, p.kd, row_bytes(p.K), p.N, p.E, BN))
     return fail(CVMM_ERR_LAUNCH, "cvmm_mx_forward: tensor map");
   if (int rc = umma::set_smem(gemm_kernel<BN, S, NACC>, L::alloc)) return rc;
   const int n_n = (int)((p.N + BN - 1) / BN);
   const unsigned grid = (unsigned)std::min<int64_t>(max_tiles * n_n, umma::sm_count());
-  launch(gemm_kernel<BN, S, NACC>, grid, kThreads, L::alloc, stream, p, a, b, n_n);
+  launch(gemm_kernel<BN, S, NACC>, grid, kThreads, L::alloc, stream, p, b, n_n);
   return check_launch("cvmm_mx_forward: gemm");
 }
 
 // Workspace of one call, in order.
 struct Sizes {
-  size_t header, cursor, tiles, list, xd, xs, y, total;
+  size_t header, cursor, tiles, list, rank, xd, xs, y, total;
   int64_t cells, max_tiles;
 };
 static Sizes sizes(int64_t x_rows, int64_t R, int64_t E, int64_t K, int64_t N, bool weighted) {
@@ -627,10 +557,11 @@ static Sizes sizes(int64_t x_rows, int64_t R, int64_t E, int64_t K, int64_t N, b
   z.cursor = align_up((size_t)E * 4, 256);
   z.tiles = align_up((size_t)z.max_tiles * sizeof(int4), 256);
   z.list = align_up((size_t)R * 4, 256);
+  z.rank = R > kPlanChunk ? align_up((size_t)R * sizeof(int2), 256) : 0;
   z.xd = align_up((size_t)(x_rows * row_bytes(K)), 256);
   z.xs = align_up((size_t)(x_rows * z.cells * 4), 256);
   z.y = weighted ? align_up((size_t)(R * N) * 2, 256) : 0;
-  z.total = z.header + z.cursor + z.tiles + z.list + z.xd + z.xs + z.y + 256;
+  z.total = z.header + z.cursor + z.tiles + z.list + z.rank + z.xd + z.xs + z.y + 256;
   return z;
 }
 
@@ -679,7 +610,7 @@ int cvmm_mx_forward(const void* x, int x_dtype, int64_t x_rows, int64_t x_ld, co
   };
   mx::Product p = {};
   p.x = x; p.x_dtype = x_dtype; p.x_rows = x_rows; p.x_ld = x_ld;
-  p.x_vec = al16(x) && x_ld * (int64_t)dtype_size(x_dtype) % 16 == 0;
+  p.x_vec = mx::vector_bytes(x, x_ld * (int64_t)dtype_size(x_dtype), 0);
   p.per_row = (int)(n_routes / x_rows);
   p.cells = z.cells;
   p.sel = sel; p.sel_dtype = sel_dtype; p.R = n_routes; p.E = (int)n_experts;
@@ -687,6 +618,7 @@ int cvmm_mx_forward(const void* x, int x_dtype, int64_t x_rows, int64_t x_ld, co
   p.cursor = reinterpret_cast<int*>(take(z.cursor));
   p.tiles = reinterpret_cast<int4*>(take(z.tiles));
   p.list = reinterpret_cast<int32_t*>(take(z.list));
+  p.rank = reinterpret_cast<int2*>(take(z.rank));
   p.xd = reinterpret_cast<uint8_t*>(take(z.xd));
   p.xs = reinterpret_cast<uint8_t*>(take(z.xs));
   p.y = reinterpret_cast<uint16_t*>(w ? take(z.y) : static_cast<char*>(out));
@@ -695,12 +627,15 @@ int cvmm_mx_forward(const void* x, int x_dtype, int64_t x_rows, int64_t x_ld, co
   p.y_vec = n_dim % 8 == 0 && al16(p.y);
 
   const int plan_blocks = (int)((n_routes + mx::kPlanChunk - 1) / mx::kPlanChunk);
-  const int quant_blocks = grid_for(x_rows * z.cells, mx::kPlanThreads / 16);
+  const int quant_blocks = grid_for(x_rows * z.cells * 4, mx::kPlanThreads);
   const size_t plan_smem = (size_t)(2 * n_experts + 1 + 34) * sizeof(int);
   if (plan_blocks > 1 && cudaMemsetAsync(p.header, 0, z.header + z.cursor, s) != cudaSuccess)
     return fail_cuda("cvmm_mx_forward: memset");
-  launch(mx::prepare_kernel, plan_blocks + quant_blocks, mx::kPlanThreads, plan_smem, s, p, plan_blocks);
-  if (plan_blocks > 1) launch(mx::fill_kernel, plan_blocks, mx::kPlanThreads, (size_t)n_experts * sizeof(int), s, p);
+  const auto prepare = x_dtype == CVMM_F32 ? mx::prepare_kernel<F32>
+                       : x_dtype == CVMM_BF16 ? mx::prepare_kernel<BF16> : mx::prepare_kernel<F16>;
+  launch(prepare, plan_blocks + quant_blocks, mx::kPlanThreads, plan_smem, s, p, plan_blocks,
+         mx::Divisor(z.cells * 4));
+  if (plan_blocks > 1) launch(mx::fill_kernel, (unsigned)((n_routes + 255) / 256), 256, 0, s, p);
   if (int rc = check_launch("cvmm_mx_forward: prepare")) return rc;
   const int64_t m_tiles = std::max(n_routes / mx::kTile, std::min(n_experts, n_routes));
   int rc;

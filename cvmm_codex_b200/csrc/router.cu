@@ -166,7 +166,7 @@ __device__ __noinline__ int decide_in_64(const Args& p, const float* z) {
 // Per round of the top-k: the largest key over the warp, then the lowest index
 // that has it, each one warp-wide integer reduction.
 template <int NPER>
-__global__ void __launch_bounds__(kWarps * 32) select_kernel(const Args p) {
+__global__ void __launch_bounds__(kWarps * 32) select_kernel(const __grid_constant__ Args p) {
   pdl_enter();
   extern __shared__ float sh[];  // per warp: logits [E], group operand [E] (with a bias or groups only)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
