@@ -126,7 +126,10 @@ def ptr(t) -> int | None:
 
 
 def stream_of(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The cudaStream_t of torch's current stream on `device`."""
+    if device.index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)  # without building a Stream object
 
 
 def device_status(reset: bool = True, device=None) -> tuple[int, int, int]:

@@ -635,8 +635,10 @@ def router_select(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bi
         if bias.device != logits.device:
             raise ValueError(f"router_select: bias is on {bias.device}, logits on {logits.device}")
         bias = bias.detach()
-    return _RouterSelect.apply(logits, int(top_k), scoring, bias, int(n_groups), int(top_groups), group_score,
-                               bool(renormalize), float(scale))
+    how = (int(top_k), scoring, bias, int(n_groups), int(top_groups), group_score, bool(renormalize), float(scale))
+    if not (torch.is_grad_enabled() and logits.requires_grad):
+        return ops.router_select(logits, *how)
+    return _RouterSelect.apply(logits, *how)
 
 
 class _RouterSelect(torch.autograd.Function):
@@ -646,13 +648,15 @@ class _RouterSelect(torch.autograd.Function):
         ctx.save_for_backward(logits, sel)
         ctx.how = (scoring, renormalize, scale)
         ctx.mark_non_differentiable(sel)
+        ctx.set_materialize_grads(False)  # no zeros for sel
         return w, sel
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_w, grad_sel):
         logits, sel = ctx.saved_tensors
-        return (ops.router_select_backward(logits, sel, grad_w, *ctx.how),) + (None,) * 8
+        grad = None if grad_w is None else ops.router_select_backward(logits, sel, grad_w, *ctx.how)
+        return (grad,) + (None,) * 8
 
 
 known_shapes = set()

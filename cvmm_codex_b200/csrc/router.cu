@@ -49,6 +49,7 @@ struct Args {
   const void* bias;  // [E] or null
   int bias_dtype;
   int G, top_groups, top2;
+  uint32_t size_inv;  // ceil(2^22 / experts of a group)
   int renorm;
   float scale;
   int64_t* sel;
@@ -74,82 +75,119 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ float warp_max(float v) {
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-
 // 1 / (1 + exp(-z)) without overflow: exp of -|z| only.
 __device__ __forceinline__ float sigmoid(float z) {
   const float e = expf(-fabsf(z));
   return (z < 0.f ? e : 1.f) / (1.f + e);
 }
 
-// Two largest values of a group, in key order.
-template <typename R>
-struct Top2 {
-  R a, b;
-  __device__ __forceinline__ void add(R v) {
-    if (key_of(v) > key_of(a)) { b = a; a = v; }
-    else if (key_of(v) > key_of(b)) b = v;
-  }
-};
-// Group value from its two largest: a masked (-inf) second counts as nothing.
-template <typename R>
-__device__ __forceinline__ R group_value(const Top2<R>& t, int top2) {
-  return top2 && t.b != -(R)INFINITY ? t.a + t.b : t.a;
+// The value of a key: the inverse of key_of up to the sign of zero and NaN bits.
+__device__ __forceinline__ float value_of(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key);
 }
 
-// Decides one token again with 64-bit scores; z: its logits in shared memory.
-// Lane j < k returns the j-th expert. Candidates are marked by bit q of `out`
-// (expert lane + 32 q already taken or outside the chosen groups).
-__device__ __noinline__ int decide_in_64(const Args& p, const float* z) {
+// Largest over the warp in one integer reduction; NaN only if every value is (as fmaxf).
+__device__ __forceinline__ float warp_max(float v) {
+  return value_of(__reduce_max_sync(0xffffffffu, v != v ? 0u : key_of(v)));
+}
+
+// Two largest values of a group, in key order, and their keys.
+template <typename R>
+struct Top2 {
+  R a = -(R)INFINITY, b = -(R)INFINITY;
+  __device__ __forceinline__ void add(R v) {
+    // NaN (above everything) compares false both ways: `!(v <= a)` takes it.
+    if (!(v <= a) && a == a) { b = a; a = v; }
+    else if (!(v <= b) && b == b) b = v;
+  }
+};
+
+// The top_groups best of p.G groups of `size` consecutive values v[e], as bits:
+// 32 / (G rounded up to a power of two) lanes share a group. worst and other:
+// the lowest chosen and the highest other group value (NaN if all are chosen).
+template <typename R>
+__device__ __forceinline__ uint32_t best_groups(const Args& p, const R* v, int size, R& worst, R& other) {
+  const int lane = threadIdx.x & 31, lanes = 32 >> (32 - __clz(p.G - 1));
+  const int g = lane / lanes;
+  Top2<R> top;
+  if (g < p.G)
+    for (int m = lane % lanes; m < size; m += lanes) top.add(v[g * size + m]);
+  for (int o = lanes >> 1; o > 0; o >>= 1) {
+    const R oa = __shfl_xor_sync(0xffffffffu, top.a, o), ob = __shfl_xor_sync(0xffffffffu, top.b, o);
+    top.add(oa);
+    top.add(ob);
+  }
+  // A masked (-inf) second counts as nothing.
+  const R gv = p.top2 && top.b != -(R)INFINITY ? top.a + top.b : top.a;
+  const auto mine = g < p.G ? key_of(gv) : 0;
+  int rank = 0;
+  uint32_t chosen = 0;
+  for (int o = 0; o < p.G; ++o) {
+    const auto k = __shfl_sync(0xffffffffu, mine, o * lanes);
+    rank += k > mine || (k == mine && o < g);
+  }
+  const uint32_t in = __ballot_sync(0xffffffffu, g < p.G && rank < p.top_groups);
+  for (int o = 0; o < p.G; ++o) chosen |= ((in >> (o * lanes)) & 1u) << o;
+  // Ranks are a permutation: exactly one group has each.
+  const uint32_t lo = __ballot_sync(0xffffffffu, g < p.G && rank == p.top_groups - 1);
+  const uint32_t hi = __ballot_sync(0xffffffffu, g < p.G && rank == p.top_groups);
+  worst = __shfl_sync(0xffffffffu, gv, __ffs(lo) - 1);
+  other = hi ? __shfl_sync(0xffffffffu, gv, __ffs(hi) - 1) : (R)NAN;
+  return chosen;
+}
+
+// e / size for e < 1024: with m = ceil(2^22 / size), e m / 2^22 is at most 2^-12
+// above e / size, less than the 1 / size to the next whole number.
+__device__ __forceinline__ int group_of(const Args& p, int e) { return (int)((uint32_t)e * p.size_inv >> 22); }
+
+__device__ __forceinline__ float logit(const Args& p, int64_t t, int e) {
+  return load_as_float(p.logits, p.dtype, t * p.ld + e);
+}
+
+// Decides token t again with 64-bit scores, kept in the warp's shared memory v
+// (E doubles). Lane j < k returns the j-th expert.
+__device__ __noinline__ int decide_in_64(const Args& p, int64_t t, double* v) {
   const int lane = threadIdx.x & 31;
   const bool softmax = p.scoring == kSoftmax;
   double mx = 0.0, sum = 1.0;
   if (softmax) {
     float m = -INFINITY;
-    for (int e = lane; e < p.E; e += 32) m = fmaxf(m, z[e]);
+    for (int e = lane; e < p.E; e += 32) m = fmaxf(m, logit(p, t, e));
     mx = warp_max(m);
     if (mx == -(double)INFINITY) mx = 0.0;
     sum = 0.0;
-    for (int e = lane; e < p.E; e += 32) sum += exp((double)z[e] - mx);
+  }
+  for (int e = lane; e < p.E; e += 32) {
+    const double z = logit(p, t, e);
+    v[e] = softmax ? exp(z - mx) : 1.0 / (1.0 + exp(-z));
+    if (softmax) sum += v[e];
+  }
+  if (softmax) {
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (sum == 0.0) sum = 1.0;
   }
-  auto by = [&](int e) -> double {
-    const double s = softmax ? exp((double)z[e] - mx) / sum : 1.0 / (1.0 + exp(-(double)z[e]));
-    const double c = p.bias ? s + (double)load_as_float(p.bias, p.bias_dtype, e) : s;
-    return z[e] == -INFINITY ? -(double)INFINITY : c;
-  };
-  auto order = [&](int e) -> double { return p.bias ? by(e) : (double)z[e]; };
-  uint32_t groups = 0xffffffffu;
-  const int size = p.E / p.G;
-  if (p.G > 1) {
-    unsigned long long mine = 0;
-    if (lane < p.G) {
-      Top2<double> t = {-(double)INFINITY, -(double)INFINITY};
-      for (int m = 0; m < size; ++m) t.add(p.top2 ? by(lane * size + m) : order(lane * size + m));
-      mine = key_of(group_value(t, p.top2));
-    }
-    int rank = 0;
-    for (int g = 0; g < p.G; ++g) {
-      const unsigned long long o = __shfl_sync(0xffffffffu, mine, g);
-      rank += o > mine || (o == mine && g < lane);
-    }
-    groups = __ballot_sync(0xffffffffu, lane < p.G && rank < p.top_groups);
+  for (int e = lane; e < p.E; e += 32) {
+    const double c = v[e] / sum + (p.bias ? (double)load_as_float(p.bias, p.bias_dtype, e) : 0.0);
+    v[e] = logit(p, t, e) == -INFINITY ? -(double)INFINITY : c;
   }
-  uint32_t out = 0;
+  __syncwarp();
+  uint32_t groups = 0xffffffffu;
+  if (p.G > 1) {
+    double worst, other;
+    groups = best_groups(p, v, p.E / p.G, worst, other);
+  }
+  uint32_t out = 0;  // bit q: expert lane + 32 q is taken or in no chosen group
   for (int q = 0; lane + 32 * q < p.E; ++q)
-    if (p.G > 1 && !((groups >> ((lane + 32 * q) / size)) & 1u)) out |= 1u << q;
+    if (p.G > 1 && !((groups >> group_of(p, lane + 32 * q)) & 1u)) out |= 1u << q;
   int chosen = 0;
   for (int j = 0; j < p.k; ++j) {
     unsigned long long best = 0;
     int be = 0x7fffffff;
     for (int q = 0; lane + 32 * q < p.E; ++q) {
       if ((out >> q) & 1u) continue;
-      const unsigned long long v = key_of(order(lane + 32 * q));
-      if (v > best) { best = v; be = lane + 32 * q; }
+      const int e = lane + 32 * q;
+      const unsigned long long key = key_of(p.bias ? v[e] : (double)logit(p, t, e));
+      if (key > best) { best = key; be = e; }
     }
     for (int o = 16; o > 0; o >>= 1) {
       const unsigned long long ov = __shfl_xor_sync(0xffffffffu, best, o);
@@ -162,31 +200,53 @@ __device__ __noinline__ int decide_in_64(const Args& p, const float* z) {
   return chosen;
 }
 
-// One warp a token; lane l holds experts l, l + 32, ... (NPER of them).
-// Per round of the top-k: the largest key over the warp, then the lowest index
-// that has it, each one warp-wide integer reduction.
+// The row of logits of token t in registers: lane l holds experts l + 32 q.
 template <int NPER>
+__device__ __forceinline__ void load_row(float (&z)[NPER], const void* logits, int dtype, int64_t at, int E) {
+  const int lane = threadIdx.x & 31;
+  if (dtype == F32) {
+#pragma unroll
+    for (int q = 0; q < NPER; ++q)
+      z[q] = lane + 32 * q < E ? static_cast<const float*>(logits)[at + lane + 32 * q] : -INFINITY;
+    return;
+  }
+  uint16_t h[NPER];
+#pragma unroll
+  for (int q = 0; q < NPER; ++q)
+    h[q] = lane + 32 * q < E ? static_cast<const uint16_t*>(logits)[at + lane + 32 * q] : 0;
+#pragma unroll
+  for (int q = 0; q < NPER; ++q) z[q] = lane + 32 * q < E ? bits_to_float(h[q], dtype) : -INFINITY;
+}
+
+// One warp a token; lane l holds experts l, l + 32, ... (NPER of them) and
+// keeps the largest of its keys. A round of the top-k is the largest key over
+// the warp, then the lowest index that has it, each one warp-wide integer
+// reduction; only the lane that gave the expert looks for its next largest.
+// BIAS and GROUPS leave out what a call without them does not do.
+template <int NPER, bool BIAS, bool GROUPS>
 __global__ void __launch_bounds__(kWarps * 32) select_kernel(const __grid_constant__ Args p) {
   pdl_enter();
-  extern __shared__ float sh[];  // per warp: logits [E], group operand [E] (with a bias or groups only)
+  extern __shared__ double sh[];  // per warp E doubles (BIAS or GROUPS only)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t t = blockIdx.x * (int64_t)kWarps + warp;
   if (t >= p.T) return;
   const int E = p.E;
   const bool softmax = p.scoring == kSoftmax;
-  float z[NPER], s[NPER];
-  float mx = -INFINITY;
+  float z[NPER], b[NPER];
+  load_row(z, p.logits, p.dtype, t * p.ld, E);
+  if (BIAS) {
 #pragma unroll
-  for (int q = 0; q < NPER; ++q) {
-    const int e = lane + 32 * q;
-    z[q] = e < E ? load_as_float(p.logits, p.dtype, t * p.ld + e) : -INFINITY;
-    mx = fmaxf(mx, z[q]);
+    for (int q = 0; q < NPER; ++q) b[q] = lane + 32 * q < E ? load_as_float(p.bias, p.bias_dtype, lane + 32 * q) : 0.f;
   }
-  float smax = 1.f;  // no score is above this
+  float mx = 0.f, sum = 1.f;
+  float s[NPER];
   if (softmax) {
+    mx = z[0];
+#pragma unroll
+    for (int q = 1; q < NPER; ++q) mx = fmaxf(mx, z[q]);
     mx = warp_max(mx);
-    if (mx == -INFINITY) mx = 0.f;  // every expert masked: all scores are 0
-    float sum = 0.f;
+    if (mx == -INFINITY || mx != mx) mx = 0.f;  // every expert masked: all scores are 0
+    sum = 0.f;
 #pragma unroll
     for (int q = 0; q < NPER; ++q) {
       s[q] = expf(z[q] - mx);
@@ -194,131 +254,84 @@ __global__ void __launch_bounds__(kWarps * 32) select_kernel(const __grid_consta
     }
     sum = warp_sum(sum);
     if (sum == 0.f) sum = 1.f;
-#pragma unroll
-    for (int q = 0; q < NPER; ++q) s[q] /= sum;
-    smax = 1.f / sum;
-  } else {
-#pragma unroll
-    for (int q = 0; q < NPER; ++q) s[q] = sigmoid(z[q]);
   }
-  float c[NPER], b[NPER];
-#pragma unroll
-  for (int q = 0; q < NPER; ++q) {
-    const int e = lane + 32 * q;
-    b[q] = p.bias && e < E ? load_as_float(p.bias, p.bias_dtype, e) : 0.f;
-    c[q] = p.bias && z[q] != -INFINITY ? s[q] + b[q] : z[q];
-  }
+  const float smax = softmax ? 1.f / sum : 1.f;  // no score is above this
   const float err = pair_error<NPER>(softmax, smax);
-  float* shz = sh + warp * 2 * E;
-  float* shv = shz + E;
-  const bool again_possible = p.bias || p.G > 1;
-  if (again_possible) {
+  if (BIAS || (GROUPS && p.top2)) {
 #pragma unroll
-    for (int q = 0; q < NPER; ++q) {
-      const int e = lane + 32 * q;
-      if (e < E) {
-        shz[e] = z[q];
-        shv[e] = p.bias || !p.top2 ? c[q] : (z[q] == -INFINITY ? -INFINITY : s[q]);
-      }
-    }
-    __syncwarp();
-  }
-  bool again = false;
-  uint32_t groups = 0xffffffffu;
-  const int size = E / p.G;
-  if (p.G > 1) {
-    // 32 / (G rounded up to a power of two) lanes share a group.
-    const int lanes = 32 >> (32 - __clz(p.G - 1));
-    const int g = lane / lanes;
-    Top2<float> top = {-INFINITY, -INFINITY};
-    if (g < p.G)
-      for (int m = lane % lanes; m < size; m += lanes) top.add(shv[g * size + m]);
-    for (int o = lanes >> 1; o > 0; o >>= 1) {
-      const float oa = __shfl_xor_sync(0xffffffffu, top.a, o), ob = __shfl_xor_sync(0xffffffffu, top.b, o);
-      top.add(oa);
-      top.add(ob);
-    }
-    const float gv = group_value(top, p.top2);
-    const uint32_t mine = g < p.G ? key_of(gv) : 0u;
-    int rank = 0;
-    for (int o = 0; o < p.G; ++o) {
-      const uint32_t v = __shfl_sync(0xffffffffu, mine, o * lanes);
-      rank += v > mine || (v == mine && o < g);
-    }
-    const bool in = g < p.G && rank < p.top_groups;
-    const uint32_t ballot = __ballot_sync(0xffffffffu, in);
-    groups = 0;
-    for (int o = 0; o < p.G; ++o) groups |= ((ballot >> (o * lanes)) & 1u) << o;
-    if (p.top_groups < p.G && (p.bias || p.top2)) {
-      // The worst chosen and the best other group must differ by more than the error of both.
-      const uint32_t lo = __reduce_min_sync(0xffffffffu, in ? mine : 0xffffffffu);
-      const uint32_t hi = __reduce_max_sync(0xffffffffu, g < p.G && !in ? mine : 0u);
-      const float worst = __shfl_sync(0xffffffffu, gv, __ffs(__ballot_sync(0xffffffffu, in && mine == lo)) - 1);
-      const float other = __shfl_sync(0xffffffffu, gv,
-                                      __ffs(__ballot_sync(0xffffffffu, g < p.G && !in && mine == hi)) - 1);
-      again = worst - other <= 2.f * err + 4.f * kAddErr * (fabsf(worst) + fabsf(other)) + kTinyErr;
-    }
+    for (int q = 0; q < NPER; ++q) s[q] = softmax ? s[q] / sum : sigmoid(z[q]);
   }
   uint32_t key[NPER];
 #pragma unroll
-  for (int q = 0; q < NPER; ++q) {
-    const int e = lane + 32 * q;
-    key[q] = e < E && (p.G == 1 || ((groups >> (e / size)) & 1u)) ? key_of(c[q]) : 0u;
-  }
-  int chosen = 0;
-  float score = 0.f;
-  float pc = 0.f, pz = 0.f, pb = 0.f;  // the expert before: c, z, b
-  const int n_cand = p.G == 1 ? E : p.top_groups * size;
-  for (int j = 0; j < n_cand; ++j) {
-    if (again || (j >= p.k && !p.bias)) break;
-    uint32_t best = 0;
-    int be = 0x7fffffff;
+  for (int q = 0; q < NPER; ++q)
+    key[q] = lane + 32 * q < E ? key_of(BIAS && z[q] != -INFINITY ? s[q] + b[q] : z[q]) : 0u;
+  bool again = false;
+  if (GROUPS) {
+    float* v = reinterpret_cast<float*>(sh + warp * E);
+#pragma unroll
+    for (int q = 0; q < NPER; ++q) {
+      const int e = lane + 32 * q;
+      if (e < E) v[e] = BIAS ? (z[q] == -INFINITY ? z[q] : s[q] + b[q]) : p.top2 && z[q] != -INFINITY ? s[q] : z[q];
+    }
+    __syncwarp();
+    float worst, other;
+    const uint32_t groups = best_groups(p, v, E / p.G, worst, other);
+    __syncwarp();
+    // The worst chosen and the best other group must differ by more than the error of both.
+    if (BIAS || p.top2)
+      again = other > -INFINITY &&
+              worst - other <= 2.f * err + 4.f * kAddErr * (fabsf(worst) + fabsf(other)) + kTinyErr;
 #pragma unroll
     for (int q = 0; q < NPER; ++q)
+      if (!((groups >> group_of(p, lane + 32 * q)) & 1u)) key[q] = 0u;
+  }
+  uint32_t best = 0;
+  int bq = 0;
+  auto local_best = [&]() {
+    best = key[0];
+    bq = 0;
+#pragma unroll
+    for (int q = 1; q < NPER; ++q)
       if (key[q] > best) {
         best = key[q];
-        be = lane + 32 * q;
+        bq = q;
       }
+  };
+  local_best();
+  int chosen = 0, last = 0;
+  float pc = 0.f;  // the value of the expert before
+  const int n_cand = GROUPS ? p.top_groups * (E / p.G) : E;
+  // With a bias one more expert is looked at, to see that it is clearly lower than the k-th.
+  int rounds = BIAS ? min(p.k + 1, n_cand) : p.k;
+  for (int j = 0; j < rounds && !again; ++j) {
     const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-    be = (int)__reduce_min_sync(0xffffffffu, best == top ? (uint32_t)be : 0xffffffffu);
-    float bs = 0.f, bc = 0.f, bz = 0.f, bb = 0.f;
-#pragma unroll
-    for (int q = 0; q < NPER; ++q)
-      if (lane + 32 * q == be) {
-        key[q] = 0;
-        bs = s[q];
-        bc = c[q];
-        bz = z[q];
-        bb = b[q];
+    const int be = (int)__reduce_min_sync(0xffffffffu, best == top ? (uint32_t)(lane + 32 * bq) : 0xffffffffu);
+    if (BIAS) {
+      // Neighbours nearer than their errors are decided again, unless they
+      // have equal logits and biases and so are equal in any number of bits.
+      const float c = value_of(top);
+      if (j > 0 && c > -INFINITY && pc - c <= err + kAddErr * (fabsf(pc) + fabsf(c)) + kTinyErr) {
+        again = logit(p, t, be) != logit(p, t, last) ||
+                load_as_float(p.bias, p.bias_dtype, be) != load_as_float(p.bias, p.bias_dtype, last);
+        if (j >= p.k) rounds = min(rounds + 1, n_cand);  // one equal to the k-th: look at the next, too
       }
-    bs = __shfl_sync(0xffffffffu, bs, be & 31);
-    if (p.bias) {
-      // Neighbours nearer than their errors are decided again, unless they are
-      // the same expert twice over (equal logit and bias: equal in any number
-      // of bits). Past the k-th the check runs on until one is clearly lower.
-      bc = __shfl_sync(0xffffffffu, bc, be & 31);
-      bz = __shfl_sync(0xffffffffu, bz, be & 31);
-      bb = __shfl_sync(0xffffffffu, bb, be & 31);
-      const bool same = bz == pz && bb == pb;
-      if (j > 0 && !same && pc - bc <= err + kAddErr * (fabsf(pc) + fabsf(bc)) + kTinyErr) again = true;
-      if (j >= p.k && !same) break;
-      pc = bc;
-      pz = bz;
-      pb = bb;
+      pc = c;
+      last = be;
     }
-    if (lane == j) {
-      chosen = be;
-      score = bs;
+    if (lane == (be & 31)) {
+#pragma unroll
+      for (int q = 0; q < NPER; ++q)
+        if (q == bq) key[q] = 0u;
+      local_best();
     }
+    if (lane == j) chosen = be;
   }
-  if (again) {
-    chosen = decide_in_64(p, shz);
-    if (lane < p.k) {
-      const float zc = shz[chosen];
-      score = softmax ? expf(zc - mx) * smax : sigmoid(zc);
-    }
+  if ((BIAS || GROUPS) && again) chosen = decide_in_64(p, t, sh + warp * E);
+  float score = 0.f;
+  if (lane < p.k) {
+    const float zc = logit(p, t, chosen);
+    score = softmax ? expf(zc - mx) / sum : sigmoid(zc);
   }
-  if (lane >= p.k) score = 0.f;
   const float tot = warp_sum(score);
   if (lane < p.k) {
     const float held = tot < 1e-20f ? 1e-20f : tot;
@@ -342,18 +355,25 @@ select_backward_kernel(const void* __restrict__ logits, int dtype, int64_t ld, c
   const int64_t t = blockIdx.x * (int64_t)kWarps + (threadIdx.x >> 5);
   if (t >= T) return;
   const bool softmax = scoring == kSoftmax;
+  int64_t e = -1;
+  float g = 0.f;
+  if (lane < k) {
+    e = sel[t * k + lane];
+    g = scale * grad_w[t * k + lane];
+    if (e < 0 || e >= E) {
+      report(CVMM_DEV_BAD_INDEX, kBadSelTag, (long long)e);
+      e = -1;
+    }
+  }
   float s[NPER];
   float mx = 0.f, inv = 1.f;
   if (softmax) {
-    mx = -INFINITY;
+    load_row(s, logits, dtype, t * ld, E);
+    mx = s[0];
 #pragma unroll
-    for (int q = 0; q < NPER; ++q) {
-      const int e = lane + 32 * q;
-      s[q] = e < E ? load_as_float(logits, dtype, t * ld + e) : -INFINITY;
-      mx = fmaxf(mx, s[q]);
-    }
+    for (int q = 1; q < NPER; ++q) mx = fmaxf(mx, s[q]);
     mx = warp_max(mx);
-    if (mx == -INFINITY) mx = 0.f;
+    if (mx == -INFINITY || mx != mx) mx = 0.f;
     float sum = 0.f;
 #pragma unroll
     for (int q = 0; q < NPER; ++q) {
@@ -363,19 +383,13 @@ select_backward_kernel(const void* __restrict__ logits, int dtype, int64_t ld, c
     sum = warp_sum(sum);
     inv = sum == 0.f ? 1.f : 1.f / sum;
   }
-  int64_t e = -1;
-  float g = 0.f, sj = 0.f, rest = 0.f;  // rest: 1 - s, from the other side
-  if (lane < k) {
-    e = sel[t * k + lane];
-    if (e < 0 || e >= E) {
-      report(CVMM_DEV_BAD_INDEX, kBadSelTag, (long long)e);
-      e = -1;
-    } else {
-      const float z = load_as_float(logits, dtype, t * ld + e);
-      sj = softmax ? expf(z - mx) * inv : sigmoid(z);
-      rest = sigmoid(-z);
-      g = scale * grad_w[t * k + lane];
-    }
+  float sj = 0.f, rest = 0.f;  // rest: 1 - s, from the other side
+  if (e >= 0) {
+    const float z = load_as_float(logits, dtype, t * ld + e);
+    sj = softmax ? expf(z - mx) * inv : sigmoid(z);
+    rest = sigmoid(-z);
+  } else {
+    g = 0.f;
   }
   if (renorm) {
     const float tot = warp_sum(sj), gs = warp_sum(g * sj);
@@ -434,12 +448,16 @@ extern "C" int cvmm_router_select(const void* logits, int logits_dtype, int64_t 
   p.E = (int)n_experts; p.k = (int)top_k; p.scoring = scoring;
   p.bias = bias; p.bias_dtype = bias_dtype;
   p.G = (int)n_groups; p.top_groups = (int)top_groups; p.top2 = group_score == CVMM_GROUP_TOP2;
+  const int64_t size = n_experts / n_groups;
+  p.size_inv = (uint32_t)((((int64_t)1 << 22) + size - 1) / size);
   p.renorm = renormalize; p.scale = scale; p.sel = sel; p.weights = weights;
   const unsigned grid = (unsigned)((n_tokens + router::kWarps - 1) / router::kWarps);
-  const size_t smem = bias || n_groups > 1 ? (size_t)router::kWarps * 2 * n_experts * sizeof(float) : 0;
+  const size_t smem = bias || n_groups > 1 ? (size_t)router::kWarps * n_experts * sizeof(double) : 0;
   return router::with_nper(n_experts, [&](auto nper) {
-    launch(router::select_kernel<decltype(nper)::value>, grid, router::kWarps * 32, smem,
-           reinterpret_cast<cudaStream_t>(stream), p);
+    constexpr int n = decltype(nper)::value;
+    const auto kernel = n_groups > 1 ? (bias ? router::select_kernel<n, true, true> : router::select_kernel<n, false, true>)
+                                     : (bias ? router::select_kernel<n, true, false> : router::select_kernel<n, false, false>);
+    launch(kernel, grid, router::kWarps * 32, smem, reinterpret_cast<cudaStream_t>(stream), p);
     return check_launch("cvmm_router_select");
   });
 }
