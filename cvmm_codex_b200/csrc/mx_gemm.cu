@@ -22,8 +22,8 @@ namespace mx {
 
 constexpr int kTile = 128;           // routes of a tile (MMA M)
 constexpr int64_t kMaxExperts = 4096;
-constexpr int kPlanThreads = 256;
-constexpr int64_t kPlanChunk = 2048;  // routes one block ranks
+constexpr int kPlanThreads = 512;
+constexpr int64_t kPlanChunk = 4096;  // routes one block ranks
 constexpr int kBadIdTag = 31;         // status-word site: an expert id outside [0, n_experts)
 enum : int { kTagEmpty = 40, kTagFull = 41, kTagAccFull = 42, kTagAccEmpty = 43, kTagDrain = 44 };
 

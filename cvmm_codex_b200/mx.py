@@ -43,17 +43,17 @@ class MXTensor:
     __slots__ = ("data", "scale", "shape", "dim")
 
     def __init__(self, data: torch.Tensor, scale: torch.Tensor, shape, dim: int = -1):
-        shape = torch.Size(shape)
+        self.shape = shape = torch.Size(shape)
+        self.data, self.scale, self.dim = data, scale, dim
         want_data, want_scale = mx_shapes(shape, dim)
-        for name, t, want in (("data", data, want_data), ("scale", scale, want_scale)):
-            if t.dtype != torch.uint8 or tuple(t.shape) != want:
-                raise ValueError(f"MXTensor: {name} must be uint8 {want} for shape {tuple(shape)}, dim {dim}; "
-                                 f"got {t.dtype} {tuple(t.shape)}")
-            if not t.is_contiguous():
-                raise ValueError(f"MXTensor: {name} must be contiguous")
+        if data.shape != want_data or scale.shape != want_scale or data.dtype != torch.uint8 or scale.dtype != torch.uint8:
+            raise ValueError(f"MXTensor: shape {tuple(shape)} quantised along dim {dim} has uint8 data {want_data} and "
+                             f"scale {want_scale}; got {data.dtype} {tuple(data.shape)} and {scale.dtype} "
+                             f"{tuple(scale.shape)}")
+        if not (data.is_contiguous() and scale.is_contiguous()):
+            raise ValueError("MXTensor: data and scale must be contiguous")
         if data.device != scale.device:
             raise ValueError("MXTensor: data and scale must be on one device")
-        self.data, self.scale, self.shape, self.dim = data, scale, shape, dim
 
     @property
     def device(self) -> torch.device:
@@ -88,7 +88,7 @@ def mx_quantize(x: torch.Tensor, dim: int = -1) -> MXTensor:
         raise ValueError(f"mx_quantize: unsupported dtype {x.dtype}")
     if dim not in (-1, -2) or x.dim() < -dim:
         raise ValueError(f"mx_quantize: dim must be -1 or -2 of a tensor that has it, got {dim} for {tuple(x.shape)}")
-    data, scale = ops.mx_quantize(x.detach(), dim)
+    data, scale = ops.mx_quantize(x.detach() if x.requires_grad else x, dim)
     return MXTensor(data, scale, x.shape, dim)
 
 
@@ -127,9 +127,10 @@ def cvmm_mx(x: torch.Tensor, sel: Union[torch.Tensor, CVMMSel], keys: MXTensor,
     if weights is not None and (tuple(weights.shape) != tuple(sel.shape) or weights.dtype not in _FLOATS):
         raise ValueError(f"cvmm_mx: weights must be a float tensor of sel's shape {tuple(sel.shape)}, "
                          f"got {weights.dtype} {tuple(weights.shape)}")
-    for name, t in (("sel", sel), ("keys", keys.data), ("weights", weights)):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"cvmm_mx: {name} is on {t.device}, x on {x.device}")
+    device = x.device
+    if sel.device != device or keys.data.device != device or (weights is not None and weights.device != device):
+        raise ValueError(f"cvmm_mx: x is on {device}, sel on {sel.device}, keys on {keys.device}"
+                         + ("" if weights is None else f", weights on {weights.device}"))
     if torch.is_grad_enabled() and (x.requires_grad or (weights is not None and weights.requires_grad)):
         raise RuntimeError("cvmm_mx has no backward: call it under torch.no_grad() or detach its inputs")
     if torch.is_autocast_enabled("cuda"):

@@ -546,9 +546,10 @@ def mx_shapes(shape, dim: int):
     return (*shape[:-2], rows, row_bytes), (*shape[:-2], *pieces)
 
 
-def _mx_strides(t: torch.Tensor, dim: int):
+def _mx_strides(t: torch.Tensor, dim: int, batch: int, rows: int, K: int):
     """(t viewed as [batch, rows, K] or copied, (batch, row, k) strides in elements)."""
-    batch, rows, K = _mx_view(t.shape, dim)
+    if t.is_contiguous():
+        return t, ((0, K, 1) if dim == -1 else (K * rows, 1, rows))
     if dim == -1:
         v = t.reshape(rows, K)
         return v, (0, v.stride(0), v.stride(1))
@@ -560,12 +561,13 @@ def mx_quantize(x: torch.Tensor, dim: int):
     """(data uint8, scale uint8) of x quantised along dim (shapes: mx_shapes)."""
     _require_cuda(x)
     lib = _lib.load()
+    dev = x.device
     data_shape, scale_shape = mx_shapes(x.shape, dim)
     batch, rows, K = _mx_view(x.shape, dim)
-    data = torch.empty(data_shape, dtype=torch.uint8, device=x.device)
-    scale = torch.empty(scale_shape, dtype=torch.uint8, device=x.device)
-    v, (sb, sr, sk) = _mx_strides(x, dim)
-    with _Device(x.device) as stream:
+    data = torch.empty(data_shape, dtype=torch.uint8, device=dev)
+    scale = torch.empty(scale_shape, dtype=torch.uint8, device=dev)
+    v, (sb, sr, sk) = _mx_strides(x, dim, batch, rows, K)
+    with _Device(dev) as stream:
         rc = _invoke("cvmm_mx_quantize", lib.cvmm_mx_quantize, ptr(v), dtype_code(v.dtype), batch, rows, K, sb, sr, sk,
                      ptr(data), ptr(scale), stream)
     check(rc, "cvmm_mx_quantize")
@@ -579,10 +581,10 @@ def mx_dequantize(data: torch.Tensor, scale: torch.Tensor, shape: Sequence[int],
     lib = _lib.load()
     batch, rows, K = _mx_view(shape, dim)
     out = torch.empty(tuple(shape), dtype=dtype, device=data.device)
-    v, (sb, sr, sk) = _mx_strides(out, dim)
+    _, (sb, sr, sk) = _mx_strides(out, dim, batch, rows, K)
     with _Device(data.device) as stream:
         rc = _invoke("cvmm_mx_dequantize", lib.cvmm_mx_dequantize, ptr(data), ptr(scale), batch, rows, K, sb, sr, sk,
-                     ptr(v), dtype_code(dtype), stream)
+                     ptr(out), dtype_code(dtype), stream)
     check(rc, "cvmm_mx_dequantize")
     return out
 
