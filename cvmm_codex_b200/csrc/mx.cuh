@@ -87,6 +87,7 @@ __device__ __forceinline__ void unpack8(uint32_t p, float (&v)[8]) {
 // below one); larger n divide.
 struct Divisor {
   uint32_t d, m, l;
+  Divisor() = default;
   __host__ explicit Divisor(int64_t by) : d((uint32_t)by), m(0), l(0) {
     while (((uint64_t)1 << l) < d) ++l;
     if (d > 1) m = (uint32_t)((((uint64_t)1 << (31 + l)) / d) + 1);

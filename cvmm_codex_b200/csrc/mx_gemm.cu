@@ -33,9 +33,9 @@ struct Product {
   int x_dtype;
   int64_t x_rows, x_ld;
   int x_vec;
-  int per_row;  // routes that share a row
+  Divisor per_row;  // routes that share a row
   uint8_t* xd;  // [x_rows][row_bytes]
-  uint8_t* xs;  // [x_rows][cells] of 4 scale bytes, cells a multiple of 4
+  uint8_t* xs;  // [x_rows][cells] of 4 scale bytes, an even number of cells
   int64_t cells;
   // routing
   const void* sel;
@@ -200,7 +200,8 @@ __global__ void __launch_bounds__(256) fill_kernel(const __grid_constant__ Produ
 //               tensor memory wants (row r's at 16 (r % 32) + 4 (r / 32)); only
 //               rows that exist. The copies arrive on the stage's barrier by
 //               themselves. (Gathers by TMA, 4 rows an instruction, took 567 us
-//               where plain rows took 403, 32768 tokens 4096 -> 512.)
+//               where plain rows took 403, 32768 tokens 4096 -> 512; arrivals a
+//               warp one or two stages late, 391 and 397 against 375.)
 //   warp 4      lane 0 loads the weight tile (TMA) and its scales (bulk copies
 //               of whole 512-byte pieces);
 //   warp 5      allocates tensor memory; lane 0 copies each stage's scales there
@@ -213,6 +214,23 @@ constexpr int kProducers = 128;
 constexpr int kLoadWarp = 4, kMmaWarp = 5, kEpilogueWarp = 6, kEpilogueWarps = 8;
 constexpr int kThreads = 32 * (kEpilogueWarp + kEpilogueWarps);
 constexpr uint32_t kStagePitch = 80;  // 64-byte row piece + 16: 16-byte accesses meet no bank twice
+
+// Position in a ring of S stages: phase is the parity of the round, which is
+// what a consumer waits for; a producer waits for the other one, and in the
+// first round for nothing.
+template <int S>
+struct Ring {
+  int s = 0;
+  uint32_t phase = 0;
+  bool first = true;
+  __device__ __forceinline__ void next() {
+    if (++s == S) {
+      s = 0;
+      phase ^= 1u;
+      first = false;
+    }
+  }
+};
 
 template <int BN, int S, int NACC>
 struct Layout {
@@ -307,27 +325,32 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ CUtensorM
     // Thread t copies 16-byte piece t % 8 of rows t / 8 + 16 i, and the scales
     // of row t. The next tile's rows are looked up during the current tile.
     const int t = threadIdx.x, piece = (t & 7) * 16;
-    auto row_of = [&](const int4& u, int i) -> int {
-      return i < u.z ? (int)((uint32_t)p.list[u.y + i] / (uint32_t)p.per_row) : -1;
-    };
-    int rows[8], next[8], srow, snext;
+    // The tile after the next is looked up, too, so that neither lookup is waited for.
     auto look = [&](const int4& u, int (&r)[8], int& sr) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r[i] = row_of(u, (t >> 3) + 16 * i);
-      sr = row_of(u, t);
+      for (int i = 0; i < 8; ++i) r[i] = (t >> 3) + 16 * i < u.z ? p.list[u.y + (t >> 3) + 16 * i] : -1;
+      sr = t < u.z ? p.list[u.y + t] : -1;
     };
-    look(tile(blockIdx.x), rows, srow);
-    uint32_t it = 0;
+    auto row_of = [&](int route) -> int { return route < 0 ? -1 : (int)p.per_row.of(route); };
+    int next[8], snext;
+    int4 un = tile(blockIdx.x + gridDim.x);
+    look(tile(blockIdx.x), next, snext);
+    Ring<S> ring;
     bool ok = true;
     for (int tt = blockIdx.x; tt < total && ok; tt += gridDim.x) {
-      look(tile(tt + gridDim.x), next, snext);
+      int rows[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) rows[i] = row_of(next[i]);
+      const int srow = row_of(snext);
+      look(un, next, snext);
+      un = tile(tt + 2 * gridDim.x);
       const uint8_t* src[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) src[i] = p.xd + (int64_t)max(rows[i], 0) * rb + piece;
       const uint8_t* scales = p.xs + (int64_t)max(srow, 0) * p.cells * 4;
-      for (int kb = 0; kb < nkb; ++kb, ++it) {
-        const int s = it % S;
-        if (it >= S && !ptx::mbar_wait_or_abort(&empty[s], ((it / S) - 1) & 1, kTagEmpty, abort)) {
+      for (int kb = 0; kb < nkb; ++kb, ring.next()) {
+        const int s = ring.s;
+        if (!ring.first && !ptx::mbar_wait_or_abort(&empty[s], ring.phase ^ 1u, kTagEmpty, abort)) {
           ok = false;
           break;
         }
@@ -344,9 +367,6 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ CUtensorM
         }
         ptx::cp_async_arrive_noinc(&full[s]);
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) rows[i] = next[i];
-      srow = snext;
     }
     ptx::cp_async_wait_all();
   } else if (warp == kLoadWarp) {
@@ -354,16 +374,16 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ CUtensorM
     if (lane == 0) {
       const int np_all = (int)pieces(p.N);
       const int64_t per_expert = scale_bytes(p.N, p.K);
-      uint32_t it = 0;
+      Ring<S> ring;
       bool ok = true;
       int4 u = tile(blockIdx.x);
       for (int tt = blockIdx.x; tt < total && ok; tt += gridDim.x) {
         const int4 un = tile(tt + gridDim.x);
         const int n0 = tt % n_n * BN, np = min(L::np, np_all - n0 / 128);
         const uint8_t* sc = p.ks + u.x * per_expert + (int64_t)(n0 / 128) * kp * kPiece;
-        for (int kb = 0; kb < nkb; ++kb, ++it) {
-          const int s = it % S;
-          if (it >= S && !ptx::mbar_wait_or_abort(&empty[s], ((it / S) - 1) & 1, kTagEmpty, abort)) {
+        for (int kb = 0; kb < nkb; ++kb, ring.next()) {
+          const int s = ring.s;
+          if (!ring.first && !ptx::mbar_wait_or_abort(&empty[s], ring.phase ^ 1u, kTagEmpty, abort)) {
             ok = false;
             break;
           }
@@ -381,8 +401,16 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ CUtensorM
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMAs
     if (lane == 0) {
+      // One thread issues everything, so its instructions a stage count: ring
+      // positions and descriptors are carried along, not computed.
+      // (Copying the scales of stage i + 1 ahead of the MMAs of stage i, or two
+      // stages' scales ahead of two stages' MMAs, was slower, 609 and 468 us:
+      // copies and MMAs drain one another.)
       const int np_all = (int)pieces(p.N);
-      uint32_t it = 0;
+      const uint64_t a0 = ptx::smem_desc_sw128(base, 16, 1024), b0 = ptx::smem_desc_sw128(base + L::a_bytes, 16, 1024);
+      const uint64_t sa0 = ptx::smem_desc_rows16(base + L::sa), sb0 = ptx::smem_desc_rows16(base + L::sb);
+      const uint32_t sf0 = tmem + NACC * BN;
+      Ring<S> ring;
       int local = 0;
       bool ok = true;
       for (int tt = blockIdx.x; tt < total && ok; tt += gridDim.x, ++local) {
@@ -390,35 +418,40 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ CUtensorM
         if (local >= NACC && !ptx::mbar_wait_or_abort(&acce[a], (local / NACC - 1) & 1, kTagAccEmpty, abort)) break;
         ptx::tc_fence_after();
         const uint32_t d = tmem + a * BN;
-        const int n0 = tt % n_n * BN, np = min(L::np, np_all - n0 / 128);
-        for (int kb = 0; kb < nkb; ++kb, ++it) {
-          const int s = it % S;
-          if (!ptx::mbar_wait_or_abort(&full[s], (it / S) & 1, kTagFull, abort)) {
+        const int n = tt % n_n, np = min(L::np, np_all - n * BN / 128);
+        // A 64-column tile reads the upper half of its 128-row scale piece at odd positions.
+        const uint32_t half = BN == 64 ? (n & 1) * 2 : 0;
+        // pc scale pieces, `steps` MMAs of K = 64; both constant but for a row's last stage.
+        auto stage = [&](int pc, int steps, bool add) {
+          const uint32_t sa = sf0 + ring.s * L::sf_cols, sb = sa + 8;
+          const uint64_t ad = a0 + ring.s * (L::stage / 16), bd = b0 + ring.s * (L::stage / 16);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            if (c >= pc) break;
+            ptx::tmem_cp_scales(sa + 4 * c, sa0 + (ring.s * 2 + c) * (kPiece / 16));
+#pragma unroll
+            for (int q = 0; q < L::np; ++q)
+              if (q < np)
+                ptx::tmem_cp_scales(sb + 4 * (c * L::np + q), sb0 + ((ring.s * L::np + q) * 2 + c) * (kPiece / 16));
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (j >= steps) break;
+            ptx::mma_mxf4(d, ad + 2 * j, bd + 2 * j, ptx::instr_desc_mxf4(kTile, BN, (j & 1) * 2), sa + 4 * (j >> 1),
+                          sb + 4 * (j >> 1) * L::np + half, add || j > 0);
+          }
+        };
+        for (int kb = 0; kb < nkb; ++kb) {
+          if (!ptx::mbar_wait_or_abort(&full[ring.s], ring.phase, kTagFull, abort)) {
             ok = false;
             break;
           }
           ptx::tc_fence_after();
           ptx::fence_proxy_async_smem();  // the rows came through the generic proxy
-          const uint32_t sa = tmem + NACC * BN + s * L::sf_cols, sb = sa + 8;
-          const int pc = min(2, kp - 2 * kb);
-          for (int c = 0; c < pc; ++c) {
-            ptx::tmem_cp_scales(sa + 4 * c, ptx::smem_desc_rows16(base + L::sa + (s * 2 + c) * kPiece));
-            for (int q = 0; q < np; ++q)
-              ptx::tmem_cp_scales(sb + 4 * (c * L::np + q),
-                                  ptx::smem_desc_rows16(base + L::sb + ((s * L::np + q) * 2 + c) * kPiece));
-          }
-          const uint32_t a_u = base + s * L::stage, b_u = a_u + L::a_bytes;
-          const int steps = min(4, (rb - kb * 128 + 31) / 32);
-          // A 64-column tile reads the upper half of its 128-row scale piece at odd positions.
-          const uint32_t half = BN == 64 ? (n0 / 64 % 2) * 2 : 0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (j < steps)
-              ptx::mma_mxf4(d, ptx::smem_desc_sw128(a_u + j * 32, 16, 1024), ptx::smem_desc_sw128(b_u + j * 32, 16, 1024),
-                            ptx::instr_desc_mxf4(kTile, BN, (j & 1) * 2), sa + 4 * (j >> 1),
-                            sb + 4 * (j >> 1) * L::np + half, (kb | j) != 0);
-          }
-          ptx::mma_commit(&empty[s]);
+          if (kb + 1 < nkb) stage(2, 4, kb != 0);
+          else stage(min(2, kp - 2 * kb), min(4, (rb - kb * 128 + 31) / 32), kb != 0);
+          ptx::mma_commit(&empty[ring.s]);
+          ring.next();
         }
         if (ok) ptx::mma_commit(&accf[a]);
       }
@@ -444,11 +477,12 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ CUtensorM
       if (!ptx::mbar_wait_or_abort(&accf[a], (local / NACC) & 1, kTagAccFull, abort)) break;
       ptx::tc_fence_after();
       uint32_t v[BN / 4];
+      const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + a * BN + group * (BN / 2);
 #pragma unroll
       for (int c = 0; c < BN / 64; ++c) {
         if (n0 + 32 * c >= p.N) break;
         float f[32];
-        umma::load_acc32(tmem + ((uint32_t)(quad * 32) << 16) + a * BN + group * (BN / 2) + 32 * c, f);
+        umma::load_acc32(from + 32 * c, f);
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[16 * c + j] = pack2(f[2 * j], f[2 * j + 1], p.out_dtype);
       }
@@ -551,7 +585,7 @@ struct Sizes {
 };
 static Sizes sizes(int64_t x_rows, int64_t R, int64_t E, int64_t K, int64_t N, bool weighted) {
   Sizes z;
-  z.cells = (pieces(K) + 3) / 4 * 4;
+  z.cells = (pieces(K) + 1) / 2 * 2;  // two a stage
   z.max_tiles = R / kTile + std::min(E, R);
   z.header = 256;
   z.cursor = align_up((size_t)E * 4, 256);
@@ -611,7 +645,7 @@ int cvmm_mx_forward(const void* x, int x_dtype, int64_t x_rows, int64_t x_ld, co
   mx::Product p = {};
   p.x = x; p.x_dtype = x_dtype; p.x_rows = x_rows; p.x_ld = x_ld;
   p.x_vec = mx::vector_bytes(x, x_ld * (int64_t)dtype_size(x_dtype), 0);
-  p.per_row = (int)(n_routes / x_rows);
+  p.per_row = mx::Divisor(n_routes / x_rows);
   p.cells = z.cells;
   p.sel = sel; p.sel_dtype = sel_dtype; p.R = n_routes; p.E = (int)n_experts;
   p.header = reinterpret_cast<int*>(take(z.header));
@@ -637,10 +671,19 @@ int cvmm_mx_forward(const void* x, int x_dtype, int64_t x_rows, int64_t x_ld, co
          mx::Divisor(z.cells * 4));
   if (plan_blocks > 1) launch(mx::fill_kernel, (unsigned)((n_routes + 255) / 256), 256, 0, s, p);
   if (int rc = check_launch("cvmm_mx_forward: prepare")) return rc;
-  const int64_t m_tiles = std::max(n_routes / mx::kTile, std::min(n_experts, n_routes));
+  // Columns of a tile: a stage takes 0.48, 0.50 and 0.67 us at 64, 128 and 256
+  // (32768 tokens 4096 -> 512: 877, 464 and 312 us), so wide tiles where they
+  // fill the SMs and narrow ones where those would leave SMs idle: 1 token 10.9,
+  // 11.3 and 13.2 us, 8 tokens 25.3, 19.0 and 13.5 us.
+  const int64_t used = std::min(n_experts, n_routes), sms = umma::sm_count();
+  const int64_t m_tiles = std::max(n_routes / mx::kTile + used / 2, used);
+  const auto cost = [&](int64_t bn, int64_t stage) {
+    return (m_tiles * ((n_dim + bn - 1) / bn) + sms - 1) / sms * stage;
+  };
+  const int64_t c64 = cost(64, 48), c128 = cost(128, 50), c256 = cost(256, 67);
   int rc;
-  if (n_dim > 128 && m_tiles * ((n_dim + 255) / 256) >= 148) rc = mx::launch_gemm<256, 4, 1>(p, z.max_tiles, s);
-  else if (n_dim > 64 && m_tiles * ((n_dim + 127) / 128) >= 148) rc = mx::launch_gemm<128, 6, 2>(p, z.max_tiles, s);
+  if (c256 < c128 && c256 < c64) rc = mx::launch_gemm<256, 4, 1>(p, z.max_tiles, s);
+  else if (c128 < c64) rc = mx::launch_gemm<128, 6, 2>(p, z.max_tiles, s);
   else rc = mx::launch_gemm<64, 7, 2>(p, z.max_tiles, s);
   if (rc || !w) return rc;
   const int64_t T = n_routes / top_k;

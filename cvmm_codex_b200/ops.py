@@ -22,7 +22,7 @@ KERNELS_PER_CALL = {
     "cvmm_weighted_token_backward": 1, "cvmm_cast": 1, "cvmm_sort_rows_padded": 2, "cvmm_sort_rows_padded_ex": 2, "cvmm_pad_starts": 1,
     "cvmm_forward_gelu": 1, "cvmm_gelu_backward": 1, "cvmm_router_topk": 1, "cvmm_padded_route_rows": 1,
     "cvmm_router_select": 1, "cvmm_router_select_backward": 1, "cvmm_mx_quantize": 1, "cvmm_mx_dequantize": 1,
-    "cvmm_mx_forward": 3,
+    "cvmm_mx_forward": 2,
 }
 
 
@@ -589,6 +589,9 @@ def mx_dequantize(data: torch.Tensor, scale: torch.Tensor, shape: Sequence[int],
     return out
 
 
+MX_PLAN_ROUTES = 4096  # kPlanChunk: routes up to which one block of the first kernel writes the experts' lists
+
+
 def mx_forward(x: torch.Tensor, sel: torch.Tensor, keys_data: torch.Tensor, keys_scale: torch.Tensor, k_dim: int,
                w: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
     """The 4-bit expert product of mx.cvmm_mx: [*sel.shape, N], or [*sel.shape[:-1], N] with w."""
@@ -605,6 +608,6 @@ def mx_forward(x: torch.Tensor, sel: torch.Tensor, keys_data: torch.Tensor, keys
         rc = _invoke("cvmm_mx_forward", lib.cvmm_mx_forward, ptr(x2), dtype_code(x2.dtype), x2.shape[0], x2.stride(0),
                      ptr(s), dtype_code(s.dtype), n_routes, k, ptr(w2), dtype_code(w2.dtype) if w2 is not None else 0,
                      ptr(keys_data), ptr(keys_scale), E, K, N, ptr(out), dtype_code(out_dtype), ptr(ws), ws.numel(),
-                     stream)
+                     stream, kernels=2 + (n_routes > MX_PLAN_ROUTES) + (w2 is not None))
     check(rc, "cvmm_mx_forward")
     return out

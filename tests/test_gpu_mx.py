@@ -275,6 +275,33 @@ def test_captured_on_other_streams_and_two_at_once():
         assert torch.equal(o1, want) and torch.equal(o2, want)
 
 
+def test_many_routes_captured():
+    """More routes than one block lists: the call's own reset of its counters is part of the graph."""
+    x, keys, sel, w = make(1700, 96, 72, 40, 3, torch.bfloat16)
+    kq = mx_quantize(keys.cuda(), dim=-2)
+    static = (x.cuda(), sel.cuda(), w.cuda())
+    want = check_product(x, keys, sel, w)
+    other = check_product(x, keys, (sel + 7) % 40, w)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = cvmm_mx(static[0], static[1], kq, static[2])
+    for s, e in ((sel, want), ((sel + 7) % 40, other), (sel, want)):
+        static[1].copy_(s)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, e)
+
+
+def test_many_experts():
+    x, keys, sel, w = make(90, 40, 24, 3000, 3, torch.float16)
+    check_product(x, keys, sel, w)
+    x, keys, sel, w = make(2000, 40, 24, 4096, 3, torch.float16)
+    check_product(x, keys, sel)
+    with pytest.raises(ValueError, match="4096"):
+        cvmm_mx(torch.zeros(1, 8, device="cuda"), torch.zeros(1, 1, dtype=torch.int64, device="cuda"),
+                mx_quantize(torch.zeros(4097, 8, 8, device="cuda"), dim=-2))
+
+
 def test_same_bits_every_time():
     x, keys, sel, w = make(900, 512, 256, 16, 4, torch.bfloat16)
     kq = mx_quantize(keys.cuda(), dim=-2)

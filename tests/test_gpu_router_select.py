@@ -137,6 +137,45 @@ def test_not_a_number_and_infinity():
             np.testing.assert_allclose(w.cpu().double().numpy(), ew, rtol=REL, atol=1e-37)
 
 
+@pytest.mark.parametrize("groups,score", [(2, "max"), (4, "max"), (4, "top2")])
+@pytest.mark.parametrize("bias", [False, True])
+def test_not_a_number_in_groups(groups, score, bias):
+    z = torch.randn(8, 20, generator=torch.Generator().manual_seed(1))
+    z[0, 7] = torch.nan
+    z[1, 3] = torch.inf
+    z[2, 5:10] = -torch.inf
+    z[2, 12] = torch.nan
+    b = torch.linspace(0, 1, 20) if bias else None
+    if bias:
+        b[17] = torch.inf
+        b[3] = -torch.inf
+    for scoring in ("softmax", "sigmoid"):
+        how = dict(scoring=scoring, n_groups=groups, top_groups=groups // 2, group_score=score)
+        w, sel = router_select(z.cuda(), 3, bias=None if b is None else b.cuda(), **how)
+        ew, es = O.select(z.double().numpy(), 3, bias=None if b is None else b.double().numpy(), **how)
+        np.testing.assert_array_equal(sel.cpu().numpy(), es)
+        np.testing.assert_allclose(w.cpu().double().numpy(), ew, rtol=REL, atol=1e-37)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_bias_types_and_strides(dtype):
+    z, b = make(50, 64, torch.float32, 12)
+    check(z, 6, scoring="sigmoid", bias=b.to(dtype))
+    wide = torch.zeros(64, 3, device="cuda")
+    wide[:, 1] = b.cuda()
+    got, want = router_select(z.cuda(), 6, bias=wide[:, 1]), router_select(z.cuda(), 6, bias=b.cuda())
+    assert all(torch.equal(a, e) for a, e in zip(got, want))
+
+
+def test_zero_bias_is_no_bias():
+    """A balance bias that starts at zero: bf16 logits tie often, and the choice is that without a bias."""
+    z, _ = make(4000, 64, torch.bfloat16, 13)
+    zero = torch.zeros(64, device="cuda")
+    for scoring in ("softmax", "sigmoid"):
+        got, want = (router_select(z.cuda(), 6, scoring=scoring, bias=b) for b in (zero, None))
+        assert torch.equal(got[1], want[1])
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renorm", [False, True])
 def test_gradient_matches_differences(scoring, renorm):
