@@ -652,11 +652,19 @@ class _RouterSelect(torch.autograd.Function):
         return w, sel
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_w, grad_sel):
-        logits, sel = ctx.saved_tensors
-        grad = None if grad_w is None else ops.router_select_backward(logits, sel, grad_w, *ctx.how)
-        return (grad,) + (None,) * 8
+        # A second derivative is refused where it would be taken (create_graph);
+        # without one the refusal's wrapper costs several microseconds a call.
+        fn = _router_select_backward_once if torch.is_grad_enabled() else _router_select_backward
+        return (fn(ctx, grad_w),) + (None,) * 8
+
+
+def _router_select_backward(ctx, grad_w):
+    logits, sel = ctx.saved_tensors
+    return None if grad_w is None else ops.router_select_backward(logits, sel, grad_w, *ctx.how)
+
+
+_router_select_backward_once = torch.autograd.function.once_differentiable(_router_select_backward)
 
 
 known_shapes = set()

@@ -589,7 +589,7 @@ def mx_dequantize(data: torch.Tensor, scale: torch.Tensor, shape: Sequence[int],
     return out
 
 
-MX_PLAN_ROUTES = 4096  # kPlanChunk: routes up to which one block of the first kernel writes the experts' lists
+MX_PLAN_ROUTES = 4096  # kPlanAlone: routes up to which one block of the first kernel writes the experts' lists
 
 
 def mx_forward(x: torch.Tensor, sel: torch.Tensor, keys_data: torch.Tensor, keys_scale: torch.Tensor, k_dim: int,
