@@ -179,8 +179,9 @@ __device__ __forceinline__ uint4 pack_block(const uint32_t (&w)[kWords<DT>], flo
 // scale needs no other lane and a row's data go out 16 bytes a lane; four lanes
 // put a 4-byte cell of scales together. at(i) gives block i; blocks of a cell
 // are consecutive and start at a multiple of 4. `first` is blocks before this
-// thread's, `stride` blocks of a round. Every lane has its loads of kBlocks
-// rounds in flight before it converts any.
+// thread's, `stride` blocks of a round. Two blocks of 16-bit values in flight a
+// lane instead of one took registers that were better spent on more warps (x of
+// 16384 x 1024: 13.7 against 8.8 us).
 struct Block {
   int64_t src;     // element offset of the row's first value
   uint8_t* data;   // the row's data bytes
@@ -192,31 +193,22 @@ struct Block {
 template <int DT, class At>
 __device__ __forceinline__ void quantize_blocks(const void* __restrict__ x, int64_t K, int vec, int64_t items,
                                                 int64_t first, int64_t stride, At at) {
-  constexpr int kBlocks = DT == F32 ? 1 : 2;
   const int lane4 = threadIdx.x & 3;
   // Every lane of a warp runs the same number of rounds (shuffles below).
-  const int64_t rounds = (items + stride * kBlocks - 1) / (stride * kBlocks);
+  const int64_t rounds = (items + stride - 1) / stride;
   for (int64_t i = 0; i < rounds; ++i) {
-    uint32_t w[kBlocks][kWords<DT>];
-    Block q[kBlocks];
-#pragma unroll
-    for (int u = 0; u < kBlocks; ++u) {
-      const int64_t it = first + (i * kBlocks + u) * stride;
-      q[u] = at(it < items ? it : 0);
-      const int64_t left = it < items && q[u].row ? K - q[u].j * 32 : 0;
-      load_block<DT>(w[u], x, q[u].src + q[u].j * 32, (int)imin64(left, 32), vec);
-    }
-#pragma unroll
-    for (int u = 0; u < kBlocks; ++u) {
-      const bool live = first + (i * kBlocks + u) * stride < items;
-      const bool in = live && q[u].row && q[u].j * 32 < K;  // this block exists
-      const uint32_t byte = in ? scale_byte(block_magnitude<DT>(w[u])) : 0u;
-      if (in) *reinterpret_cast<uint4*>(q[u].data + q[u].j * 16) = pack_block<DT>(w[u], inverse_scale(byte));
-      uint32_t cell = byte << (8 * lane4);
-      cell |= __shfl_xor_sync(0xffffffffu, cell, 1);
-      cell |= __shfl_xor_sync(0xffffffffu, cell, 2);
-      if (live && lane4 == 0) *q[u].cell = cell;
-    }
+    const int64_t it = first + i * stride;
+    const bool live = it < items;
+    const Block q = at(live ? it : 0);
+    const bool in = live && q.row && q.j * 32 < K;  // this block exists
+    uint32_t w[kWords<DT>];
+    load_block<DT>(w, x, q.src + q.j * 32, in ? (int)imin64(K - q.j * 32, 32) : 0, vec);
+    const uint32_t byte = in ? scale_byte(block_magnitude<DT>(w)) : 0u;
+    if (in) *reinterpret_cast<uint4*>(q.data + q.j * 16) = pack_block<DT>(w, inverse_scale(byte));
+    uint32_t cell = byte << (8 * lane4);
+    cell |= __shfl_xor_sync(0xffffffffu, cell, 1);
+    cell |= __shfl_xor_sync(0xffffffffu, cell, 2);
+    if (live && lane4 == 0) *q.cell = cell;
   }
 }
 
