@@ -39,7 +39,7 @@ __device__ __forceinline__ float pair_error(bool softmax, float smax) {
   return softmax ? smax * (1.3e-6f + 6e-8f * (EPL + 5)) : 9e-7f;
 }
 constexpr float kAddErr = 6e-8f;   // relative, of c
-constexpr float kTinyErr = 1e-38f; // scores below the normal range
+constexpr float kTinyErr = 1e-37f; // scores below the normal range, which __expf gives as 0 (1.2e-38 each)
 
 enum Scoring : int { kSoftmax = CVMM_SCORE_SOFTMAX, kSigmoid = CVMM_SCORE_SIGMOID };
 
@@ -369,10 +369,22 @@ __global__ void __launch_bounds__(kWarps * 32) select_kernel(const __grid_consta
       worst |= __shfl_xor_sync(0xffffffffu, worst, o);
       other |= __shfl_xor_sync(0xffffffffu, other, o);
     }
-    // The worst chosen and the best other group must differ by more than the error of both.
+    // The worst chosen and the best other group must differ by more than the
+    // error of both. With a bias a value is a sum of up to two c, which may be
+    // large with a small sum: half an ulp of each c (at most 1 + max |b|) and of
+    // each sum (at most twice that), for two groups.
     const float lo = value_of(worst), hi = value_of(other);
-    if ((BIAS || p.top2) && p.top_groups < p.G)
-      again = hi > -INFINITY && lo - hi <= 2.f * err + 4.f * kAddErr * (fabsf(lo) + fabsf(hi)) + kTinyErr;
+    if ((BIAS || p.top2) && p.top_groups < p.G) {
+      float size_c = fabsf(lo) + fabsf(hi);
+      if (BIAS) {
+        size_c = 0.f;
+#pragma unroll
+        for (int q = 0; q < EPL; ++q)
+          if (fabsf(b[q]) < INFINITY) size_c = fmaxf(size_c, fabsf(b[q]));
+        size_c = 2.f * (1.f + token_max<LPT>(size_c));
+      }
+      again = hi > -INFINITY && lo - hi <= 2.f * err + 4.f * kAddErr * size_c + kTinyErr;
+    }
 #pragma unroll
     for (int q = 0; q < EPL; ++q)
       if (!((chosen >> (group_of(p, min(e0 + q, E - 1)) & 31)) & 1u)) key[q] = 0u;

@@ -157,6 +157,22 @@ def test_not_a_number_in_groups(groups, score, bias):
         np.testing.assert_allclose(w.cpu().double().numpy(), ew, rtol=REL, atol=1e-37)
 
 
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups,score", [(1, "max"), (8, "max"), (8, "top2"), (32, "top2")])
+@pytest.mark.parametrize("size", [1e3, 1e6])
+def test_large_biases_of_both_signs(scoring, groups, score, size):
+    """Biases whose 32-bit sums with a score lose the score: groups of a large and a large negative one, nearly equal."""
+    T, E = 300, 64
+    g = torch.Generator().manual_seed(17)
+    z = torch.randn(T, E, generator=g)
+    bias = size * (1 + torch.rand(E // 2, generator=g))
+    bias = torch.stack((bias, -bias), dim=1).flatten()
+    check(z, 4, scoring=scoring, bias=bias, n_groups=groups, top_groups=max(1, groups // 2), group_score=score)
+    off = bias.clone()
+    off[::5] = -torch.inf
+    check(z, 4, scoring=scoring, bias=off, n_groups=groups, top_groups=max(1, groups // 2), group_score=score)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_bias_types_and_strides(dtype):
     z, b = make(50, 64, torch.float32, 12)
