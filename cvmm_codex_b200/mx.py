@@ -37,7 +37,8 @@ class MXTensor:
            unflattened, [*shape[:-1], 16 * ceil(K / 32)]);
     scale: uint8 [*leading, ceil(rows / 128), ceil(K / 128), 32, 4, 4], the scale
            2^(byte - 127) of row r, group j at [r // 128, j // 4, r % 32,
-           r % 128 // 32, j % 4]; 255 marks a group that held an infinity or NaN.
+           r % 128 // 32, j % 4]; 255 marks a group that held an infinity or
+           NaN; bytes of rows and groups that do not exist are 0.
     """
 
     __slots__ = ("data", "scale", "shape", "dim")
@@ -88,8 +89,10 @@ def mx_quantize(x: torch.Tensor, dim: int = -1) -> MXTensor:
         raise ValueError(f"mx_quantize: unsupported dtype {x.dtype}")
     if dim not in (-1, -2) or x.dim() < -dim:
         raise ValueError(f"mx_quantize: dim must be -1 or -2 of a tensor that has it, got {dim} for {tuple(x.shape)}")
-    data, scale = ops.mx_quantize(x.detach() if x.requires_grad else x, dim)
-    return MXTensor(data, scale, x.shape, dim)
+    q = MXTensor.__new__(MXTensor)  # nothing to check
+    q.data, q.scale = ops.mx_quantize(x.detach() if x.requires_grad else x, dim)
+    q.shape, q.dim = x.shape, dim
+    return q
 
 
 def cvmm_mx(x: torch.Tensor, sel: Union[torch.Tensor, CVMMSel], keys: MXTensor,

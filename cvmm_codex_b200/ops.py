@@ -113,6 +113,17 @@ class _Device:
         return False
 
 
+def _call(name, fn, device: torch.device, *args, kernels=None):
+    """fn(*args, stream) on the current stream of `device`; raises on a bad status."""
+    if _recorder is None and torch._C._cuda_getDevice() == device.index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with _Device(device) as stream:
+            rc = _invoke(name, fn, *args, stream, kernels=kernels)
+    if rc:
+        check(rc, name)
+
+
 # ------------------------------------------------------------------ selector prep
 def sel_prepare(sel: torch.Tensor, top_k: int, route_input: bool):
     """Stable expert sort of routes (reference cvmm_prepare_sel2, cvmm.py:1786-1803).
@@ -497,14 +508,11 @@ def router_select(logits: torch.Tensor, top_k: int, scoring: str, bias: Optional
     lg = _rows(logits)
     T, E = lg.shape
     b = None if bias is None else bias.contiguous()
-    sel = torch.empty((*logits.shape[:-1], int(top_k)), dtype=torch.int64, device=lg.device)
-    w = torch.empty((*logits.shape[:-1], int(top_k)), dtype=torch.float32, device=lg.device)
-    with _Device(lg.device) as stream:
-        rc = _invoke("cvmm_router_select", lib.cvmm_router_select, ptr(lg), dtype_code(lg.dtype), lg.stride(0), T, E,
-                     int(top_k), SCORING[scoring], ptr(b), dtype_code(b.dtype) if b is not None else 0, int(n_groups),
-                     int(top_groups), GROUP_SCORE[group_score], int(bool(renormalize)), float(scale), ptr(sel), ptr(w),
-                     stream)
-    check(rc, "cvmm_router_select")
+    shape = (*logits.shape[:-1], int(top_k))
+    sel, w = lg.new_empty(shape, dtype=torch.int64), lg.new_empty(shape, dtype=torch.float32)
+    _call("cvmm_router_select", lib.cvmm_router_select, lg.device, ptr(lg), dtype_code(lg.dtype), lg.stride(0), T, E,
+          int(top_k), SCORING[scoring], ptr(b), dtype_code(b.dtype) if b is not None else 0, int(n_groups),
+          int(top_groups), GROUP_SCORE[group_score], int(bool(renormalize)), float(scale), ptr(sel), ptr(w))
     return w, sel
 
 
@@ -517,11 +525,9 @@ def router_select_backward(logits: torch.Tensor, sel: torch.Tensor, grad_w: torc
     T, E = lg.shape
     s, g = sel.contiguous(), grad_w.float().contiguous()
     out = torch.empty(logits.shape, dtype=lg.dtype, device=lg.device)
-    with _Device(lg.device) as stream:
-        rc = _invoke("cvmm_router_select_backward", lib.cvmm_router_select_backward, ptr(lg), dtype_code(lg.dtype),
-                     lg.stride(0), ptr(s), ptr(g), T, E, sel.shape[-1], SCORING[scoring], int(bool(renormalize)),
-                     float(scale), ptr(out), stream)
-    check(rc, "cvmm_router_select_backward")
+    _call("cvmm_router_select_backward", lib.cvmm_router_select_backward, lg.device, ptr(lg), dtype_code(lg.dtype),
+          lg.stride(0), ptr(s), ptr(g), T, E, sel.shape[-1], SCORING[scoring], int(bool(renormalize)),
+          float(scale), ptr(out))
     return out
 
 
@@ -567,10 +573,8 @@ def mx_quantize(x: torch.Tensor, dim: int):
     data = torch.empty(data_shape, dtype=torch.uint8, device=dev)
     scale = torch.empty(scale_shape, dtype=torch.uint8, device=dev)
     v, (sb, sr, sk) = _mx_strides(x, dim, batch, rows, K)
-    with _Device(dev) as stream:
-        rc = _invoke("cvmm_mx_quantize", lib.cvmm_mx_quantize, ptr(v), dtype_code(v.dtype), batch, rows, K, sb, sr, sk,
-                     ptr(data), ptr(scale), stream)
-    check(rc, "cvmm_mx_quantize")
+    _call("cvmm_mx_quantize", lib.cvmm_mx_quantize, dev, ptr(v), dtype_code(v.dtype), batch, rows, K, sb, sr, sk,
+          ptr(data), ptr(scale))
     return data, scale
 
 
@@ -582,10 +586,8 @@ def mx_dequantize(data: torch.Tensor, scale: torch.Tensor, shape: Sequence[int],
     batch, rows, K = _mx_view(shape, dim)
     out = torch.empty(tuple(shape), dtype=dtype, device=data.device)
     _, (sb, sr, sk) = _mx_strides(out, dim, batch, rows, K)
-    with _Device(data.device) as stream:
-        rc = _invoke("cvmm_mx_dequantize", lib.cvmm_mx_dequantize, ptr(data), ptr(scale), batch, rows, K, sb, sr, sk,
-                     ptr(out), dtype_code(dtype), stream)
-    check(rc, "cvmm_mx_dequantize")
+    _call("cvmm_mx_dequantize", lib.cvmm_mx_dequantize, data.device, ptr(data), ptr(scale), batch, rows, K, sb, sr, sk,
+          ptr(out), dtype_code(dtype))
     return out
 
 
@@ -604,10 +606,8 @@ def mx_forward(x: torch.Tensor, sel: torch.Tensor, keys_data: torch.Tensor, keys
     k, n_routes = s.shape[-1], s.numel()
     out = torch.empty((*(s.shape if w is None else s.shape[:-1]), N), dtype=out_dtype, device=x.device)
     ws = _ws(lib.cvmm_mx_workspace_size(x2.shape[0], n_routes, E, K, N, int(w is not None)), x.device)
-    with _Device(x.device) as stream:
-        rc = _invoke("cvmm_mx_forward", lib.cvmm_mx_forward, ptr(x2), dtype_code(x2.dtype), x2.shape[0], x2.stride(0),
-                     ptr(s), dtype_code(s.dtype), n_routes, k, ptr(w2), dtype_code(w2.dtype) if w2 is not None else 0,
-                     ptr(keys_data), ptr(keys_scale), E, K, N, ptr(out), dtype_code(out_dtype), ptr(ws), ws.numel(),
-                     stream, kernels=2 + (n_routes > MX_PLAN_ROUTES) + (w2 is not None))
-    check(rc, "cvmm_mx_forward")
+    _call("cvmm_mx_forward", lib.cvmm_mx_forward, x.device, ptr(x2), dtype_code(x2.dtype), x2.shape[0], x2.stride(0),
+          ptr(s), dtype_code(s.dtype), n_routes, k, ptr(w2), dtype_code(w2.dtype) if w2 is not None else 0,
+          ptr(keys_data), ptr(keys_scale), E, K, N, ptr(out), dtype_code(out_dtype), ptr(ws), ws.numel(),
+          kernels=2 + (n_routes > MX_PLAN_ROUTES) + (w2 is not None))
     return out
