@@ -63,6 +63,13 @@ __device__ __forceinline__ uint32_t pack8(const float (&v)[8], float inv) {
   return out;
 }
 
+// The value of one code (sign, two exponent bits, one more bit).
+__device__ __forceinline__ float value_of_code(uint32_t c) {
+  const uint32_t m = c & 7u;
+  const uint32_t bits = m >= 2u ? ((126u + (m >> 1)) << 23) | ((m & 1u) << 22) : m ? 0x3f000000u : 0u;
+  return __uint_as_float(bits | (c & 8u) << 28);
+}
+
 // The eight values of four packed bytes.
 __device__ __forceinline__ void unpack8(uint32_t p, float (&v)[8]) {
   uint32_t h[4];
