@@ -105,8 +105,8 @@ def cvmm_mx(x: torch.Tensor, sel: Union[torch.Tensor, CVMMSel], keys: MXTensor,
     int64), or a CVMMSel, whose raw_sel and reduction_weight are used. keys:
     mx_quantize(w, dim=-2) of w [E, K, N]. weights: [..., k] route weights of the
     weighted sum over k. Returns [..., k, N], or [..., N] with weights, in
-    autocast's dtype, else x's (bfloat16 for a float32 x). Route outputs are
-    rounded to that dtype before the weighted sum, which is held in 32 bits."""
+    autocast's dtype, else x's (bfloat16 for a float32 x). Route outputs and
+    their weighted sum are held in 32 bits and rounded to that dtype once."""
     if isinstance(sel, CVMMSel):
         if weights is not None and sel.reduction_weight is not None:
             raise ValueError("cvmm_mx: weights given twice (argument and CVMMSel.reduction_weight)")

@@ -400,7 +400,7 @@ int cvmm_mx_dequantize(const uint8_t* data, const uint8_t* scale, int64_t n_batc
 
 /* Expert product of 4-bit rows with 4-bit weights, for serving (no backward):
  *   y[r] = Q(x[r / (n_routes / x_rows)]) . W[sel[r]]^T     fp32 accumulate
- *   out[r] = y[r], or with w out[t] = sum_j w[t,j] y[t top_k + j]   (fp32 sum)
+ *   out[r] = y[r], or with w out[t] = sum_j w[t,j] y[t top_k + j]   (fp32, rounded once)
  * Q quantises a row of x as cvmm_mx_quantize does. W is a microscaled tensor of
  * n_experts x n_dim rows of k_dim (keys [E, k, n] quantised along k).
  * x: [x_rows, k_dim] fp32/bf16/fp16 with leading dimension x_ld, x_rows a

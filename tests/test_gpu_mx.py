@@ -330,3 +330,35 @@ def test_kept_weights_round_trip():
     r = MXTensor(q.data.cpu().cuda(), q.scale.clone(), q.shape, dim=-2)
     assert torch.equal(r.dequantize(), q.dequantize()) and r.to("cpu").device.type == "cpu"
     assert repr(r).startswith("MXTensor(") and b.MXTensor is MXTensor
+
+
+# ------------------------------------------------------------------ weighted sums are rounded once
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows", ["token", "route"])
+@pytest.mark.parametrize("T,K,N,E,k", [(32, 512, 1024, 128, 8), (3, 200, 74, 7, 4), (33, 31, 5, 3, 2), (500, 96, 260, 5, 3),
+                                       (700, 160, 640, 4, 5), (9000, 64, 128, 5, 3), (9000, 64, 100, 5, 3)])
+def test_weighted_sum_is_rounded_once(dtype, rows, T, K, N, E, k):
+    """`expected`'s tolerance without half a step of every route output: the sums alone, and one rounding."""
+    x, keys, sel, w = make(T, K, N, E, k, dtype, rows, seed=T + N)
+    out = cvmm_mx(x.cuda(), sel.cuda(), mx_quantize(keys.cuda(), dim=-2), w.cuda())
+    xq = O.mx_values(*O.mx_quantize(view3(x, -1)), K)[0]
+    wq = O.mx_values(*O.mx_quantize(view3(keys, -2)), K)
+    exact, size, y = O.mx_product(xq, sel.numpy(), wq, w.double().numpy(), 1 if rows == "route" else k)
+    route = (np.abs(y) * w.double().numpy()[..., None]).sum(-2)
+    half = torch.finfo(out.dtype).eps / 2
+    low = 2.0 ** -25 if out.dtype == torch.float16 else 1e-37
+    tol = ((K / 32 + 8) * size + (k + 1) * route) * 2.0 ** -23 * (1 + half) + half * np.abs(exact) + low
+    err = np.abs(out.cpu().double().numpy() - exact)
+    assert (err <= tol).all(), f"{(err / tol).max()} of the tolerance"
+
+
+@pytest.mark.parametrize("N", [8, 36, 37, 300, 640])
+def test_weighted_sum_of_routes_past_the_16_bit_range(N):
+    """Two routes of 64 * 256 * 4 = 65536, which fp16 does not hold, with weights 1/4 and 1/2: 49152 exactly."""
+    x = torch.full((3, 64), 256.0, dtype=torch.float16, device="cuda")
+    keys = mx_quantize(torch.full((2, 64, N), 4.0, device="cuda"), dim=-2)
+    sel = torch.tensor([[0, 1], [1, 0], [1, 1]], device="cuda")
+    w = torch.tensor([0.25, 0.5], device="cuda").expand(3, 2)
+    out = cvmm_mx(x, sel, keys, w)
+    assert out.dtype == torch.float16 and torch.equal(out, torch.full((3, N), 49152.0, dtype=torch.float16, device="cuda"))
+    assert torch.isinf(cvmm_mx(x, sel, keys)).all()
