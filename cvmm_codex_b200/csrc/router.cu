@@ -26,17 +26,16 @@ constexpr int kWarps = 4;
 constexpr int kBadSelTag = 30;  // status-word site: a chosen id outside [0, n_experts)
 
 // How far the difference of two 32-bit values may be from the exact one.
-// __expf(-x) is within 2 + 1.17 x ulp of 1.2e-7, and (2 + 1.17 x) e^-x <= 2.4.
-// Softmax, in units of the largest score 1 / sum: that, 2.9e-7, the argument's
-// half ulp, x e^-x 6e-8 <= 2.2e-8, and the product with the rounded 1 / sum,
-// 1.8e-7, for each of the two; the sum's error scales the whole difference,
-// which is at most one unit: EPL additions in a lane and 5 across at 6e-8 and
-// its terms' 2.9e-7. Sigmoid, each: s (1 - s) times the first, 9e-8, half an
-// ulp of 1 + e and 2 ulp of the division, 3e-7. c = s + b adds half an ulp of
-// each c.
+// Softmax, in units of the largest score 1 / sum: expf's 2 ulp of 1.2e-7, the
+// argument's half ulp, x e^-x 6e-8 <= 2.2e-8, and the product with the rounded
+// 1 / sum, 1.8e-7, for each of the two; the sum's error scales the whole
+// difference, which is at most one unit: EPL additions in a lane and 5 across at
+// 6e-8 and its terms' 2.4e-7. Sigmoid takes __expf(-x), within 2 + 1.17 x ulp,
+// and (2 + 1.17 x) e^-x <= 2.4: each s (1 - s) times that, 9e-8, half an ulp of
+// 1 + e and 2 ulp of the division, 3e-7. c = s + b adds half an ulp of each c.
 template <int EPL>
 __device__ __forceinline__ float pair_error(bool softmax, float smax) {
-  return softmax ? smax * (1.3e-6f + 6e-8f * (EPL + 5)) : 9e-7f;
+  return softmax ? smax * (1.2e-6f + 6e-8f * (EPL + 5)) : 9e-7f;
 }
 constexpr float kAddErr = 6e-8f;   // relative, of c
 constexpr float kTinyErr = 1e-37f; // scores below the normal range, which __expf gives as 0 (1.2e-38 each)
@@ -316,7 +315,7 @@ __global__ void __launch_bounds__(kWarps * 32) select_kernel(const __grid_consta
     float sum = 0.f;
 #pragma unroll
     for (int q = 0; q < EPL; ++q) {
-      s[q] = __expf(z[q] - mx);
+      s[q] = expf(z[q] - mx);  // the sum is the weights' and the gradient's, too
       sum += e0 + q < E ? s[q] : 0.f;
     }
     sum = token_sum<LPT>(sum);

@@ -311,3 +311,15 @@ def test_traces_without_a_graph_break():
     assert torch.equal(cs, sel) and torch.equal(cw, w)
     g = torch.randn_like(w)
     assert torch.equal(torch.autograd.grad(cw, zc, g)[0], torch.autograd.grad(w, zc, g)[0])
+
+
+@pytest.mark.parametrize("E", [6, 64, 100, 300, 1000])
+@pytest.mark.parametrize("bias", [False, True])
+def test_weights_and_gradient_share_their_scores(E, bias):
+    """One expert a token, no renormalising: the gradient at it is w (1 - w) of the very weight returned."""
+    z, b = make(400, E, torch.float32, E, bias)
+    zc = (3 * z).cuda().requires_grad_(True)
+    w, sel = router_select(zc, 1, bias=None if b is None else b.cuda(), renormalize=False)
+    (gz,) = torch.autograd.grad(w, zc, torch.ones_like(w))
+    w = w.detach()
+    assert torch.equal(gz.gather(-1, sel), w * (1 - w))
