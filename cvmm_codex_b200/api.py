@@ -597,6 +597,11 @@ class _RouterTopK(torch.autograd.Function):
         return gl.to(logits.dtype), None, None
 
 
+def has_tangent(t: torch.Tensor) -> bool:
+    """Whether t carries a forward-mode tangent, which a kernel call would drop."""
+    return torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+
+
 def router_select(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias: Optional[torch.Tensor] = None,
                   n_groups: int = 1, top_groups: Optional[int] = None, group_score: str = "max",
                   renormalize: bool = True, scale: float = 1.0):
@@ -613,7 +618,8 @@ def router_select(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bi
     scores. weights: the unbiased scores of the chosen, divided by their sum
     when renormalize (held at 1e-20), times scale. Experts with logit -inf are
     chosen after all others, with weight 0; NaN logits rank first and give NaN
-    weights. Differentiable once w.r.t. the logits. No reference counterpart
+    weights. Differentiable once w.r.t. the logits, in reverse mode; a logits
+    tensor with a forward-mode tangent is refused. No reference counterpart
     beyond softmax top-k (router_topk)."""
     if logits.dim() < 1 or logits.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise ValueError(f"router_select: logits must be a float tensor [..., E], got {logits.dtype} {tuple(logits.shape)}")
@@ -635,6 +641,8 @@ def router_select(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bi
         if bias.device != logits.device:
             raise ValueError(f"router_select: bias is on {bias.device}, logits on {logits.device}")
         bias = bias.detach()
+    if has_tangent(logits):
+        raise NotImplementedError("router_select has no forward-mode derivative")
     how = (int(top_k), scoring, bias, int(n_groups), int(top_groups), group_score, bool(renormalize), float(scale))
     if not (torch.is_grad_enabled() and logits.requires_grad):
         return ops.router_select(logits, *how)

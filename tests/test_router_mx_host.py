@@ -139,3 +139,17 @@ def test_oracle_quantisation_is_nearest():
     step = np.where(a < 2, 0.5, np.where(a < 4, 1.0, 2.0))
     assert (np.abs(v - x) / s <= np.where(a > 6, a - 6, step / 2)).all()
     assert a.max() < 8
+
+
+def test_router_select_refuses_a_tangent():
+    """A forward-mode derivative is refused, not dropped, with gradients enabled or not."""
+    z, t = torch.randn(4, 8), torch.randn(4, 8)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(z, t)
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
+                b.router_select(dual, 2)
+        with pytest.raises(RuntimeError, match="CUDA"):  # a tensor without a tangent is none of its business
+            b.router_select(z, 2)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda a: b.router_select(a, 2)[0], (z,), (t,))
