@@ -20,7 +20,7 @@ from typing import Optional, Union
 import torch
 
 from ._torch_ops import calls as ops
-from .api import CVMMSel
+from .api import CVMMSel, has_tangent
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -136,6 +136,8 @@ def cvmm_mx(x: torch.Tensor, sel: Union[torch.Tensor, CVMMSel], keys: MXTensor,
                          + ("" if weights is None else f", weights on {weights.device}"))
     if torch.is_grad_enabled() and (x.requires_grad or (weights is not None and weights.requires_grad)):
         raise RuntimeError("cvmm_mx has no backward: call it under torch.no_grad() or detach its inputs")
+    if has_tangent(x) or (weights is not None and has_tangent(weights)):
+        raise NotImplementedError("cvmm_mx has no forward-mode derivative")
     if torch.is_autocast_enabled("cuda"):
         out_dtype = torch.get_autocast_dtype("cuda")
     else:

@@ -153,3 +153,15 @@ def test_router_select_refuses_a_tangent():
             b.router_select(z, 2)
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(lambda a: b.router_select(a, 2)[0], (z,), (t,))
+
+
+def test_cvmm_mx_refuses_tangents():
+    x, sel, w = torch.zeros(4, 40), torch.zeros(4, 2, dtype=torch.int64), torch.ones(4, 2)
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for args in ((dual(x), sel, _keys()), (dual(x), sel, _keys(), w), (x, sel, _keys(), dual(w)),
+                     (x, b.CVMMSel(sel.int(), sel.int(), sel.reshape(-1), None, dual(w)), _keys())):
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                b.cvmm_mx(*args)
+        with pytest.raises(RuntimeError, match="CUDA"):
+            b.cvmm_mx(x, sel, _keys(), w)
