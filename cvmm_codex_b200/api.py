@@ -661,18 +661,29 @@ class _RouterSelect(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_w, grad_sel):
-        # A second derivative is refused where it would be taken (create_graph);
-        # without one the refusal's wrapper costs several microseconds a call.
-        fn = _router_select_backward_once if torch.is_grad_enabled() else _router_select_backward
-        return (fn(ctx, grad_w),) + (None,) * 8
+        if grad_w is None:
+            return (None,) * 9
+        logits, sel = ctx.saved_tensors
+        # Only a graph of the gradient (create_graph) needs the node that refuses
+        # the second derivative; it costs several microseconds a call. Compiled
+        # graphs refuse it themselves.
+        if torch.is_grad_enabled() and not torch.compiler.is_compiling():
+            grad = _RouterSelectGrad.apply(logits, sel, grad_w, *ctx.how)
+        else:
+            grad = ops.router_select_backward(logits, sel, grad_w, *ctx.how)
+        return (grad,) + (None,) * 8
 
 
-def _router_select_backward(ctx, grad_w):
-    logits, sel = ctx.saved_tensors
-    return None if grad_w is None else ops.router_select_backward(logits, sel, grad_w, *ctx.how)
+class _RouterSelectGrad(torch.autograd.Function):
+    """The gradient as a function of the logits and grad_w both, so that no second derivative passes it by."""
 
+    @staticmethod
+    def forward(ctx, logits, sel, grad_w, scoring, renormalize, scale):
+        return ops.router_select_backward(logits, sel, grad_w, scoring, renormalize, scale)
 
-_router_select_backward_once = torch.autograd.function.once_differentiable(_router_select_backward)
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("router_select is differentiable once: its gradient has no derivative")
 
 
 known_shapes = set()

@@ -165,3 +165,39 @@ def test_cvmm_mx_refuses_tangents():
                 b.cvmm_mx(*args)
         with pytest.raises(RuntimeError, match="CUDA"):
             b.cvmm_mx(x, sel, _keys(), w)
+
+
+@pytest.fixture
+def router_on_the_cpu(monkeypatch):
+    """The two router calls replaced by the 64-bit oracle, so that autograd's part runs without a GPU."""
+    from cvmm_codex_b200 import api
+
+    def select(self, logits, k, scoring, bias, n_groups, top_groups, group_score, renormalize, scale):
+        w, sel = O.select(logits.detach().numpy(), k, scoring, bias, n_groups, top_groups, group_score, renormalize, scale)
+        return torch.from_numpy(w).float(), torch.from_numpy(sel)
+
+    def backward(self, logits, sel, grad_w, scoring, renormalize, scale):
+        g, _ = O.select_grad(logits.detach().double().numpy(), sel.numpy(), grad_w.detach().numpy(), scoring,
+                             renormalize, scale)
+        return torch.from_numpy(g).to(logits.dtype)
+
+    monkeypatch.setattr(type(api.ops), "router_select", select)
+    monkeypatch.setattr(type(api.ops), "router_select_backward", backward)
+
+
+def test_a_linear_loss_has_no_second_derivative_either(router_on_the_cpu):
+    """The weights' gradient depends on the logits even where the loss's own does not: refused, not left out."""
+    r = torch.randn(3, 2)
+    for loss in (lambda w: (w * r).sum(), lambda w: w.square().sum()):
+        z = torch.randn(3, 8, requires_grad=True)
+        (g,) = torch.autograd.grad(loss(b.router_select(z, 2)[0]), z, create_graph=True)
+        assert g.requires_grad
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            (g.square().sum() + z.square().sum()).backward()
+    z = torch.randn(3, 8, requires_grad=True)
+    (g,) = torch.autograd.grad((b.router_select(z, 2)[0] * r).sum(), z)
+    assert not g.requires_grad
+    w, sel = b.router_select(z, 2)
+    (w * r).sum().backward(create_graph=True)  # a graph that nobody differentiates
+    assert torch.equal(z.grad, g)
+    assert torch.autograd.grad((z.sum() * 2), z)[0].eq(2).all()
