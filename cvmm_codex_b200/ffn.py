@@ -111,7 +111,8 @@ class SigmaMoEFFNMX(torch.nn.Module):
 
     Made by SigmaMoEFFN.quantized(), a copy of that layer as it is then. The
     weights' bytes, the gate and the bias are buffers: they move with the
-    module and are in its state_dict. Forward only, without gradients."""
+    module and are in its state_dict. Forward only: an input that requires grad
+    is refused while gradients are recorded, as cvmm_mx refuses it."""
 
     def __init__(self, layer: SigmaMoEFFN):
         super().__init__()
@@ -124,7 +125,6 @@ class SigmaMoEFFNMX(torch.nn.Module):
             self.register_buffer(name + "_data", q.data)
             self.register_buffer(name + "_scale", q.scale)
 
-    @torch.no_grad()
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return sigma_moe_ffn(x, self.gate, MXTensor(self.up_data, self.up_scale, self.up_shape, dim=-2),
                              MXTensor(self.down_data, self.down_scale, self.down_shape, dim=-2), self.k,

@@ -128,3 +128,14 @@ def test_mixed_weights_are_refused():
     with pytest.raises(ValueError, match="both"):
         sigma_moe_ffn(x, layer.gate, mx_quantize(layer.w_up, dim=-2), layer.w_down, 6)
     assert isinstance(mx_quantize(layer.w_up, dim=-2), MXTensor)
+
+
+def test_served_layer_refuses_a_gradient():
+    layer, x = layer_and_input(T=20, **ROUTING)
+    served = layer.quantized()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        want = served(x)
+        with pytest.raises(RuntimeError, match="no backward"):
+            served(x.clone().requires_grad_(True))
+        with torch.no_grad():
+            assert torch.equal(served(x.clone().requires_grad_(True)), want)

@@ -201,3 +201,25 @@ def test_a_linear_loss_has_no_second_derivative_either(router_on_the_cpu):
     (w * r).sum().backward(create_graph=True)  # a graph that nobody differentiates
     assert torch.equal(z.grad, g)
     assert torch.autograd.grad((z.sum() * 2), z)[0].eq(2).all()
+
+
+def test_the_served_layer_refuses_a_gradient(monkeypatch):
+    """An input's gradient is refused, not dropped; without one, or under no_grad, the layer gets to its product."""
+    from cvmm_codex_b200 import api
+
+    def quantize(self, x, dim):
+        return tuple(torch.zeros(s, dtype=torch.uint8) for s in mx_shapes(x.shape, dim))
+
+    def topk(self, logits, k, renormalize):
+        return torch.ones(*logits.shape[:-1], k), torch.zeros(*logits.shape[:-1], k, dtype=torch.int64)
+
+    monkeypatch.setattr(type(api.ops), "mx_quantize", quantize)
+    monkeypatch.setattr(type(api.ops), "router_topk", topk)
+    served = b.SigmaMoEFFN(16, 4, 8, 2).quantized()
+    x = torch.randn(3, 16)
+    with pytest.raises(RuntimeError, match="no backward"):
+        served(x.clone().requires_grad_(True))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        served(x)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+        served(x.clone().requires_grad_(True))
