@@ -58,7 +58,9 @@ def sigma_moe_ffn(x: torch.Tensor, gate: torch.Tensor, w_up: Weights, w_down: We
     if mx != isinstance(w_down, MXTensor):
         raise ValueError("sigma_moe_ffn: w_up and w_down must both be MXTensors or both be tensors")
     logits = x @ gate
-    if scoring == "softmax" and bias is None and n_groups == 1 and scale == 1.0:
+    # Arguments that router_select refuses go to it even where router_topk would not look at them.
+    plain = scoring == "softmax" and bias is None and n_groups == 1 and scale == 1.0
+    if plain and top_groups in (None, 1) and group_score in ("max", "top2"):
         weights, sel = router_topk(logits, k, renormalize)
     else:
         weights, sel = router_select(logits, k, scoring=scoring, bias=bias, n_groups=n_groups, top_groups=top_groups,

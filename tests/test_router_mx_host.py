@@ -223,3 +223,16 @@ def test_the_served_layer_refuses_a_gradient(monkeypatch):
         served(x)
     with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
         served(x.clone().requires_grad_(True))
+
+
+@pytest.mark.parametrize("bad", [dict(top_groups=2), dict(top_groups=0), dict(group_score="sum"), dict(scoring="tanh"),
+                                 dict(n_groups=3), dict(bias=torch.zeros(3))])
+def test_the_layer_refuses_what_its_router_refuses(bad):
+    x, gate = torch.zeros(5, 16), torch.zeros(16, 4)
+    with pytest.raises(ValueError, match="router_select"):
+        b.sigma_moe_ffn(x, gate, torch.zeros(4, 16, 8), torch.zeros(4, 8, 16), 2, **bad)
+    layer = b.SigmaMoEFFN(16, 4, 8, 2, **{k: v for k, v in bad.items() if k != "bias"})
+    if "bias" in bad:
+        layer.bias = bad["bias"]
+    with pytest.raises(ValueError, match="router_select"):
+        layer(x)
