@@ -82,10 +82,12 @@ def _require_cuda(*ts):
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """2-D row-major view [rows, cols] with unit column stride."""
+    """2-D row-major view [rows, cols] with unit column stride and a row stride of at least cols."""
     t2 = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
     if t2.stride(-1) != 1 or (t2.shape[0] > 1 and t2.stride(0) < t2.shape[1]):
         t2 = t2.contiguous()
+    if t2.stride(0) < t2.shape[1]:  # a single row may have any row stride (a transposed column's is 1)
+        t2 = t2.as_strided(t2.shape, (t2.shape[1], 1))
     return t2
 
 

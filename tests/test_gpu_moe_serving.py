@@ -139,3 +139,26 @@ def test_served_layer_refuses_a_gradient():
             served(x.clone().requires_grad_(True))
         with torch.no_grad():
             assert torch.equal(served(x.clone().requires_grad_(True)), want)
+
+
+def test_one_token_from_a_transposed_product():
+    """A [1, n] tensor of strides (1, 1) gives what its copy gives: routing and its gradient, and the expert products."""
+    from cvmm_codex_b200 import cvmm_mx
+    torch.manual_seed(2)
+    x = torch.randn(64, 1, device="cuda").bfloat16().T
+    gate, w = torch.randn(64, 16, device="cuda").bfloat16(), torch.randn(16, 64, 48, device="cuda") / 8
+    logits = (gate.T @ x.T).T
+    assert x.stride() == (1, 1) and logits.stride() == (1, 1)
+    outs = []
+    for same in (lambda t: t.detach(), lambda t: t.detach().reshape(-1).clone().view(1, -1)):
+        z = same(logits).requires_grad_(True)
+        weights, sel = router_select(z, 4, scoring="sigmoid", bias=torch.zeros(16, device="cuda"))
+        (gz,) = torch.autograd.grad(weights, z, torch.arange(4.0, device="cuda").view(1, 4))
+        t = same(x).requires_grad_(True)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            y = cvmm(t, cvmm_prepare_sel2(sel), w)
+        g = torch.linspace(-1, 1, 48, device="cuda").bfloat16().view(48, 1).T.expand(4, 48).view(1, 4, 48)
+        (gx,) = torch.autograd.grad(y, t, g)
+        outs.append((weights.detach(), sel, gz, y.detach(), gx, cvmm_mx(same(x), sel, mx_quantize(w, dim=-2)),
+                     cvmm_mx(same(x), sel, mx_quantize(w, dim=-2), weights.detach())))
+    assert all(torch.equal(a, e) for a, e in zip(*outs))

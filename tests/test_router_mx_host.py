@@ -236,3 +236,24 @@ def test_the_layer_refuses_what_its_router_refuses(bad):
         layer.bias = bad["bias"]
     with pytest.raises(ValueError, match="router_select"):
         layer(x)
+
+
+@pytest.mark.parametrize("rows", [0, 1, 2])
+def test_single_rows_of_any_stride_reach_the_library_with_a_whole_row_stride(rows, monkeypatch):
+    """A transposed column [1, E] has strides (1, 1) and torch calls it contiguous."""
+    from cvmm_codex_b200 import ops
+    seen = []
+    monkeypatch.setattr(ops, "_require_cuda", lambda *t: None)
+    monkeypatch.setattr(ops, "_call", lambda name, fn, device, *args, **kw: seen.append((name, args)))
+    x = torch.randn(40, rows).T
+    sel = torch.zeros(rows, 2, dtype=torch.int64)
+    if rows < 2:
+        assert x.stride(0) < 40 and x.is_contiguous()
+    ops.router_select(x, 2, "softmax", None, 1, 1, "max", True, 1.0)
+    ops.router_select_backward(x, sel, torch.zeros(rows, 2), "softmax", True, 1.0)
+    k = _keys()
+    ops.mx_forward(x, sel, k.data, k.scale, 40, None, torch.bfloat16)
+    ld = {"cvmm_router_select": 2, "cvmm_router_select_backward": 2, "cvmm_mx_forward": 3}
+    assert len(seen) == 3 and all(args[ld[name]] >= 40 for name, args in seen)
+    v = torch.arange(6.0).view(6, 1)[1:].T
+    assert torch.equal(ops._rows(v), v) and ops._rows(v).stride() == (5, 1) and ops._rows(v).data_ptr() == v.data_ptr()
