@@ -73,10 +73,6 @@ __device__ __forceinline__ unsigned long long key_of(double v) {
   return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
 // 1 / (1 + exp(-z)) without overflow: exp of -|z| only. FAST where an error in
 // s of 3e-7 will do, else relative.
 template <bool FAST = false>
