@@ -618,6 +618,17 @@ static int launch_gemm(const Product& p, int64_t max_tiles, cudaStream_t stream)
   return check_launch("cvmm_mx_forward: gemm");
 }
 
+// Columns of a tile: a stage takes 0.48, 0.50 and 0.67 us at 64, 128 and 256
+// (32768 tokens 4096 -> 512: 877, 464 and 312 us), so wide tiles where they
+// fill the SMs and narrow ones where those would leave SMs idle: 1 token 10.9,
+// 11.3 and 13.2 us, 8 tokens 25.3, 19.0 and 13.5 us.
+static int tile_columns(int64_t R, int64_t E, int64_t N, int64_t sms) {
+  const int64_t used = std::min(E, R), m_tiles = std::max(R / kTile + used / 2, used);
+  const auto cost = [&](int64_t bn, int64_t stage) { return (m_tiles * ((N + bn - 1) / bn) + sms - 1) / sms * stage; };
+  const int64_t c64 = cost(64, 48), c128 = cost(128, 50), c256 = cost(256, 67);
+  return c256 < c128 && c256 < c64 ? 256 : c128 < c64 ? 128 : 64;
+}
+
 // Workspace of one call, in order.
 struct Sizes {
   size_t header, cursor, tiles, list, rank, xd, xs, y, total;
@@ -648,6 +659,11 @@ size_t cvmm_mx_workspace_size(int64_t x_rows, int64_t n_routes, int64_t n_expert
                               int weighted) {
   if (x_rows < 0 || n_routes < 0 || n_experts < 0 || k_dim < 0 || n_dim < 0) return 0;
   return cvmm::mx::sizes(x_rows, n_routes, n_experts, k_dim, n_dim, weighted != 0).total;
+}
+
+int cvmm_mx_tile_columns(int64_t n_routes, int64_t n_experts, int64_t n_dim, int64_t sms) {
+  if (n_routes < 1 || n_experts < 1 || n_dim < 1 || sms < 1) return 0;
+  return cvmm::mx::tile_columns(n_routes, n_experts, n_dim, sms);
 }
 
 int cvmm_mx_forward(const void* x, int x_dtype, int64_t x_rows, int64_t x_ld, const void* sel, int sel_dtype,
@@ -713,20 +729,10 @@ int cvmm_mx_forward(const void* x, int x_dtype, int64_t x_rows, int64_t x_ld, co
          mx::Divisor(z.cells * 4));
   if (plan_blocks > 1) launch(mx::fill_kernel, (unsigned)((n_routes + 255) / 256), 256, 0, s, p);
   if (int rc = check_launch("cvmm_mx_forward: prepare")) return rc;
-  // Columns of a tile: a stage takes 0.48, 0.50 and 0.67 us at 64, 128 and 256
-  // (32768 tokens 4096 -> 512: 877, 464 and 312 us), so wide tiles where they
-  // fill the SMs and narrow ones where those would leave SMs idle: 1 token 10.9,
-  // 11.3 and 13.2 us, 8 tokens 25.3, 19.0 and 13.5 us.
-  const int64_t used = std::min(n_experts, n_routes), sms = umma::sm_count();
-  const int64_t m_tiles = std::max(n_routes / mx::kTile + used / 2, used);
-  const auto cost = [&](int64_t bn, int64_t stage) {
-    return (m_tiles * ((n_dim + bn - 1) / bn) + sms - 1) / sms * stage;
-  };
-  const int64_t c64 = cost(64, 48), c128 = cost(128, 50), c256 = cost(256, 67);
-  int rc;
-  if (c256 < c128 && c256 < c64) rc = mx::launch_gemm<256, 4, 1>(p, z.max_tiles, s);
-  else if (c128 < c64) rc = mx::launch_gemm<128, 6, 2>(p, z.max_tiles, s);
-  else rc = mx::launch_gemm<64, 7, 2>(p, z.max_tiles, s);
+  const int columns = mx::tile_columns(n_routes, n_experts, n_dim, umma::sm_count());
+  const int rc = columns == 256   ? mx::launch_gemm<256, 4, 1>(p, z.max_tiles, s)
+                 : columns == 128 ? mx::launch_gemm<128, 6, 2>(p, z.max_tiles, s)
+                                  : mx::launch_gemm<64, 7, 2>(p, z.max_tiles, s);
   if (rc || !w) return rc;
   const int64_t T = n_routes / top_k;
   launch(mx::combine_kernel, (unsigned)((T * ((n_dim + 7) / 8) + 255) / 256), 256, 0, s,

@@ -362,3 +362,17 @@ def test_weighted_sum_of_routes_past_the_16_bit_range(N):
     out = cvmm_mx(x, sel, keys, w)
     assert out.dtype == torch.float16 and torch.equal(out, torch.full((3, N), 49152.0, dtype=torch.float16, device="cuda"))
     assert torch.isinf(cvmm_mx(x, sel, keys)).all()
+
+
+# T, K, N, E, k, weighted: several 128-column tiles, whole and ragged, one and two tiles an SM
+COLUMNS_128 = [(1600, 160, 384, 8, 3, False), (1600, 288, 370, 8, 3, True), (1600, 96, 200, 8, 3, True),
+               (1600, 31, 374, 8, 3, False), (3300, 544, 384, 8, 3, False), (3300, 160, 380, 8, 3, True)]
+
+
+@pytest.mark.parametrize("T,K,N,E,k,weighted", COLUMNS_128)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_product_of_several_128_column_tiles(T, K, N, E, k, weighted, dtype):
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert _lib.load().cvmm_mx_tile_columns(T * k, E, N, sms) == 128
+    x, keys, sel, w = make(T, K, N, E, k, dtype, seed=N)
+    check_product(x, keys, sel, w if weighted else None)

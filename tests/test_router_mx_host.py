@@ -257,3 +257,13 @@ def test_single_rows_of_any_stride_reach_the_library_with_a_whole_row_stride(row
     assert len(seen) == 3 and all(args[ld[name]] >= 40 for name, args in seen)
     v = torch.arange(6.0).view(6, 1)[1:].T
     assert torch.equal(ops._rows(v), v) and ops._rows(v).stride() == (5, 1) and ops._rows(v).data_ptr() == v.data_ptr()
+
+
+@pytest.mark.parametrize("routes,experts,n,columns", [
+    (8, 128, 512, 64), (64, 128, 512, 256), (262144, 128, 512, 256), (65536, 64, 128, 128), (0, 8, 8, 0), (8, 8, 0, 0),
+    # the shapes of test_gpu_mx.COLUMNS_128
+    (4800, 8, 384, 128), (4800, 8, 370, 128), (4800, 8, 200, 128), (4800, 8, 374, 128), (9900, 8, 384, 128),
+    (9900, 8, 380, 128),
+])
+def test_tile_columns(routes, experts, n, columns):
+    assert _lib.load().cvmm_mx_tile_columns(routes, experts, n, 148) == columns
