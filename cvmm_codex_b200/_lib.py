@@ -70,6 +70,7 @@ SIGNATURES = {
     "cvmm_mx_quantize": (_I, [_P, _I, _L, _L, _L, _L, _L, _L, _P, _P, _P]),
     "cvmm_mx_dequantize": (_I, [_P, _P, _L, _L, _L, _L, _L, _L, _P, _I, _P]),
     "cvmm_mx_workspace_size": (_S, [_L, _L, _L, _L, _L, _I]),
+    "cvmm_mx_launches": (_I, [_L, _I]),
     "cvmm_mx_tile_columns": (_I, [_L, _L, _L, _L]),
     "cvmm_mx_forward": (_I, [_P, _I, _L, _L, _P, _I, _L, _L, _P, _I, _P, _P, _L, _L, _L, _P, _I, _P, _S, _P]),
 }

@@ -661,6 +661,10 @@ size_t cvmm_mx_workspace_size(int64_t x_rows, int64_t n_routes, int64_t n_expert
   return cvmm::mx::sizes(x_rows, n_routes, n_experts, k_dim, n_dim, weighted != 0).total;
 }
 
+int cvmm_mx_launches(int64_t n_routes, int weighted) {
+  return n_routes <= 0 ? 0 : 2 + (n_routes > cvmm::mx::kPlanAlone) + (weighted != 0);
+}
+
 int cvmm_mx_tile_columns(int64_t n_routes, int64_t n_experts, int64_t n_dim, int64_t sms) {
   if (n_routes < 1 || n_experts < 1 || n_dim < 1 || sms < 1) return 0;
   return cvmm::mx::tile_columns(n_routes, n_experts, n_dim, sms);

@@ -593,9 +593,6 @@ def mx_dequantize(data: torch.Tensor, scale: torch.Tensor, shape: Sequence[int],
     return out
 
 
-MX_PLAN_ROUTES = 4096  # kPlanAlone: routes up to which one block of the first kernel writes the experts' lists
-
-
 def mx_forward(x: torch.Tensor, sel: torch.Tensor, keys_data: torch.Tensor, keys_scale: torch.Tensor, k_dim: int,
                w: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
     """The 4-bit expert product of mx.cvmm_mx: [*sel.shape, N], or [*sel.shape[:-1], N] with w."""
@@ -611,5 +608,5 @@ def mx_forward(x: torch.Tensor, sel: torch.Tensor, keys_data: torch.Tensor, keys
     _call("cvmm_mx_forward", lib.cvmm_mx_forward, x.device, ptr(x2), dtype_code(x2.dtype), x2.shape[0], x2.stride(0),
           ptr(s), dtype_code(s.dtype), n_routes, k, ptr(w2), dtype_code(w2.dtype) if w2 is not None else 0,
           ptr(keys_data), ptr(keys_scale), E, K, N, ptr(out), dtype_code(out_dtype), ptr(ws), ws.numel(),
-          kernels=2 + (n_routes > MX_PLAN_ROUTES) + (w2 is not None))
+          kernels=None if _recorder is None else lib.cvmm_mx_launches(n_routes, int(w2 is not None)))
     return out

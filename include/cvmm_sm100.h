@@ -409,7 +409,9 @@ int cvmm_mx_dequantize(const uint8_t* data, const uint8_t* scale, int64_t n_batc
  * out: bf16/fp16, contiguous. */
 size_t cvmm_mx_workspace_size(int64_t x_rows, int64_t n_routes, int64_t n_experts, int64_t k_dim, int64_t n_dim,
                               int weighted);
-/* Columns of the product's tiles (64, 128 or 256) on a device of `sms` multiprocessors. */
+/* Kernels that one cvmm_mx_forward call launches, and the columns of its product's
+ * tiles (64, 128 or 256) on a device of `sms` multiprocessors. */
+int cvmm_mx_launches(int64_t n_routes, int weighted);
 int cvmm_mx_tile_columns(int64_t n_routes, int64_t n_experts, int64_t n_dim, int64_t sms);
 int cvmm_mx_forward(const void* x, int x_dtype, int64_t x_rows, int64_t x_ld, const void* sel, int sel_dtype,
                     int64_t n_routes, int64_t top_k, const void* w, int w_dtype, const uint8_t* keys_data,

@@ -376,3 +376,14 @@ def test_product_of_several_128_column_tiles(T, K, N, E, k, weighted, dtype):
     assert _lib.load().cvmm_mx_tile_columns(T * k, E, N, sms) == 128
     x, keys, sel, w = make(T, K, N, E, k, dtype, seed=N)
     check_product(x, keys, sel, w if weighted else None)
+
+
+@pytest.mark.parametrize("T,weighted", [(4, False), (4, True), (2000, False), (2000, True)])
+def test_recorded_launches(T, weighted):
+    from cvmm_codex_b200 import ops
+    x, keys, sel, w = make(T, 64, 48, 4, 3, torch.bfloat16)
+    kq, args = mx_quantize(keys.cuda(), dim=-2), (x.cuda(), sel.cuda(), w.cuda() if weighted else None)
+    rec = ops.Recorder()
+    with rec:
+        cvmm_mx(args[0], args[1], kq, args[2])
+    assert rec.launches == 2 + (T * 3 > 4096) + weighted

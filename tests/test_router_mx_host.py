@@ -267,3 +267,8 @@ def test_single_rows_of_any_stride_reach_the_library_with_a_whole_row_stride(row
 ])
 def test_tile_columns(routes, experts, n, columns):
     assert _lib.load().cvmm_mx_tile_columns(routes, experts, n, 148) == columns
+
+
+def test_launches():
+    lib = _lib.load()
+    assert [lib.cvmm_mx_launches(r, w) for r, w in ((0, 1), (1, 0), (4096, 1), (4097, 0), (4097, 1))] == [0, 2, 3, 3, 4]
