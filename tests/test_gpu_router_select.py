@@ -323,3 +323,12 @@ def test_weights_and_gradient_share_their_scores(E, bias):
     (gz,) = torch.autograd.grad(w, zc, torch.ones_like(w))
     w = w.detach()
     assert torch.equal(gz.gather(-1, sel), w * (1 - w))
+
+
+def test_compiled_and_linear_losses_have_no_second_derivative_either():
+    r = torch.randn(3, 2, device="cuda")
+    for fn in (lambda t: router_select(t, 2)[0], torch.compile(lambda t: router_select(t, 2)[0], fullgraph=True)):
+        z = torch.randn(3, 8, device="cuda", requires_grad=True)
+        with pytest.raises(RuntimeError):
+            (g,) = torch.autograd.grad((fn(z) * r).sum(), z, create_graph=True)
+            (g.square().sum() + z.square().sum()).backward()
