@@ -12,7 +12,14 @@
 // Computing every c in 64 bits would cost more than all the rest; instead the
 // order is taken from 32-bit values whose error is bounded, every pair of
 // neighbours in it is checked against that bound, and only a token with a pair
-// nearer than the bound (about one in a thousand) is decided again in 64 bits.
+// nearer than the bound is decided again in 64 bits. How many that are depends
+// on the inputs (64 experts top 4 and 128 experts top 8, logits of deviation
+// 1.5): 0.01 to 0.1 % with a bias of deviation 0.05. A zero bias leaves equal
+// logits equal, and a tie between the k-th and the next expert always goes there:
+// 3.4 and 7.3 % with bf16 logits, 1 % with fp16. The bound of a sigmoid is
+// absolute, so with a zero bias scores near 0 or 1 go there, too: 95 % at logits
+// around -14, 29 % around +6. 32768 tokens x 128 experts, bf16 softmax: 20.3 us
+// without a bias, 29.4 with one, 45.1 with a zero one.
 #include "common.cuh"
 #include "launch.h"
 

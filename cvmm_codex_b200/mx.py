@@ -4,7 +4,8 @@
 consecutive values share one power-of-two scale, and each value is held in 4
 bits (0, 0.5, 1, 1.5, 2, 3, 4 or 6 times the scale, with a sign). Expert
 weights kept this way take 17/64 of their bf16 bytes, and the sm_100a tensor
-cores multiply them without unpacking, at four times the bf16 rate.
+cores multiply them without unpacking, at nominally four times the bf16 rate
+(measured in the product's kernel: 3.5 PFLOP/s, twice a bf16 library product's).
 
     w_up_mx = mx_quantize(w_up, dim=-2)         # [E, K, N], once, at load
     y = cvmm_mx(x, sel, w_up_mx)                # as cvmm(x, sel, w_up), forward only
