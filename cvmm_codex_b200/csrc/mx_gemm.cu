@@ -55,7 +55,7 @@ struct Product {
   const uint8_t* ks;
   int64_t K, N;
   void* y;  // route outputs: 16-bit in out_dtype, or 32-bit for combine
-  bool y32;
+  int64_t y_words;  // 16-bit words of a row of y: N, or 2 N
   int out_dtype;
   bool y_vec;
 };
@@ -66,12 +66,11 @@ __device__ __forceinline__ int64_t expert_of(const Product& p, int64_t r) {
 }
 
 // A route whose id names no expert: reported, and its output is zero.
+// What it needs of registers prepare_kernel reserves (a choice by width here made
+// that 47 for 40, two blocks an SM for three: 65 us for 57, 32768 tokens x 4096).
 __device__ __noinline__ void bad_route(const Product& p, int64_t r, int64_t e) {
   report(CVMM_DEV_BAD_INDEX, kBadIdTag, (long long)e);
-  for (int64_t n = 0; n < p.N; ++n) {
-    if (p.y32) static_cast<float*>(p.y)[r * p.N + n] = 0.f;
-    else static_cast<uint16_t*>(p.y)[r * p.N + n] = 0;
-  }
+  for (int64_t n = 0; n < p.y_words; ++n) static_cast<uint16_t*>(p.y)[r * p.y_words + n] = 0;
 }
 
 // From counts[E] in shared memory: counts[e] becomes the start of expert e's
@@ -217,10 +216,9 @@ __global__ void __launch_bounds__(256) fill_kernel(const __grid_constant__ Produ
 //   warps 6-13  two groups read half the accumulator's columns each, round them
 //               into registers, hand the accumulator back and only then store,
 //               through shared memory in 64-byte row pieces. 32-bit outputs, twice
-//               the registers, are stored 32 columns at a time straight from them,
-//               and the accumulator goes back after the last load (32 tokens 512 ->
-//               4096, the whole call: 33.5 us; through shared memory, with the
-//               accumulator held meanwhile, 52.4).
+//               the registers, are stored 32 columns at a time straight from them
+//               before the accumulator goes back (32 tokens 512 -> 4096, the whole
+//               call: 32 us; through shared memory, 52).
 constexpr int kProducers = 128;
 constexpr int kLoadWarp = 4, kMmaWarp = 5, kEpilogueWarp = 6, kEpilogueWarps = 8;
 constexpr int kThreads = 32 * (kEpilogueWarp + kEpilogueWarps);
@@ -502,35 +500,28 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ CUtensorM
       const int64_t n0 = (int64_t)(tt % n_n) * BN + group * (BN / 2);
       if (!ptx::mbar_wait_or_abort(&accf[a], (local / NACC) & 1, kTagAccFull, abort)) break;
       ptx::tc_fence_after();
+      uint32_t v[WIDE ? 32 : BN / 4];
       const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + a * BN + group * (BN / 2);
-      const int64_t off = route < 0 ? -1 : (int64_t)route * p.N + n0;
-      auto hand_back = [&]() {
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&acce[a]);
-      };
-      if constexpr (WIDE) {
-        const int chunks = (int)min((int64_t)(BN / 64), max((int64_t)0, (p.N - n0 + 31) / 32));
-        if (chunks == 0) hand_back();
-        for (int c = 0; c < chunks; ++c) {
-          uint32_t r[32];
-          ptx::tmem_ld_32x32b_x32(from + 32 * c, r);
-          ptx::tmem_wait_ld();
-          if (c + 1 == chunks) hand_back();
-          store_rows(static_cast<float*>(p.y), off < 0 ? -1 : off + 32 * c, r, (int)imin64(32, p.N - n0 - 32 * c),
-                     p.y_vec);
-        }
-      } else {
-        uint32_t v[BN / 4];
 #pragma unroll
-        for (int c = 0; c < BN / 64; ++c) {
-          if (n0 + 32 * c >= p.N) break;
+      for (int c = 0; c < BN / 64; ++c) {
+        if (n0 + 32 * c >= p.N) break;
+        if constexpr (WIDE) {
+          ptx::tmem_ld_32x32b_x32(from + 32 * c, v);
+          ptx::tmem_wait_ld();
+          store_rows(static_cast<float*>(p.y), route < 0 ? -1 : (int64_t)route * p.N + n0 + 32 * c, v,
+                     (int)imin64(32, p.N - n0 - 32 * c), p.y_vec);
+        } else {
           float f[32];
           umma::load_acc32(from + 32 * c, f);
 #pragma unroll
           for (int j = 0; j < 16; ++j) v[16 * c + j] = pack2(f[2 * j], f[2 * j + 1], p.out_dtype);
         }
-        hand_back();
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&acce[a]);
+      if constexpr (!WIDE) {
+        const int64_t off = route < 0 ? -1 : (int64_t)route * p.N + n0;
 #pragma unroll
         for (int c = 0; c < BN / 64; ++c) {
           if (n0 + 32 * c >= p.N) break;
@@ -610,7 +601,7 @@ static int launch_gemm(const Product& p, int64_t max_tiles, cudaStream_t stream)
   CUtensorMap b;
   if (!weights_map(&b, p.kd, row_bytes(p.K), p.N, p.E, BN))
     return fail(CVMM_ERR_LAUNCH, "cvmm_mx_forward: tensor map");
-  const auto kernel = p.y32 ? gemm_kernel<BN, S, NACC, true> : gemm_kernel<BN, S, NACC, false>;
+  const auto kernel = p.y_words != p.N ? gemm_kernel<BN, S, NACC, true> : gemm_kernel<BN, S, NACC, false>;
   if (int rc = umma::set_smem(kernel, L::alloc)) return rc;
   const int n_n = (int)((p.N + BN - 1) / BN);
   const unsigned grid = (unsigned)std::min<int64_t>(max_tiles * n_n, umma::sm_count());
@@ -716,7 +707,7 @@ int cvmm_mx_forward(const void* x, int x_dtype, int64_t x_rows, int64_t x_ld, co
   p.xd = reinterpret_cast<uint8_t*>(take(z.xd));
   p.xs = reinterpret_cast<uint8_t*>(take(z.xs));
   p.y = w ? take(z.y) : out;
-  p.y32 = w != nullptr;
+  p.y_words = w ? 2 * n_dim : n_dim;
   p.kd = keys_data; p.ks = keys_scale; p.K = k_dim; p.N = n_dim;
   p.out_dtype = out_dtype;
   p.y_vec = n_dim % 8 == 0 && al16(p.y);
